@@ -231,6 +231,11 @@ def _lib() -> ctypes.CDLL:
         lib.rl_moe_table_route.argtypes = [P, P, I, I, I, I, F, P, P, P, P, P, P, P, P, I, P, P]
         lib.rl_gated_join_norm.argtypes = [P, L, F, P, L, F, P, L, P, P, P, L, P, L, I, I, F, F, P]
         lib.rl_bias_kv_store.argtypes = [I, P, L, P, L, P, P, I, P, P, L, P, P, P, I, I, I, I, I, I, I, I, P, P]
+        lib.rl_kv8_write.argtypes = [I, P, L, P, L, P, P, P, I, I, P, P, P, P, I, I, I, I, I, I, I, P, P]
+        lib.rl_kv8_attention.argtypes = [I, P, L, P, P, P, I, I, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, P, P, P, P]
+        lib.rl_copy_pages.argtypes = [P, P, I, P, I, I, P, P]
+        for name in ("rl_kv8_write", "rl_kv8_attention", "rl_copy_pages"):
+            getattr(lib, name).restype = I
         for name in ("rl_rmsnorm", "rl_rmsnorm_add", "rl_cast_rows", "rl_latent_attention_fits", "rl_latent_decode_fits",
                      "rl_latent_kv_write", "rl_latent_q_rope", "rl_latent_attention", "rl_head_linear", "rl_gated_act",
                      "rl_token_gate", "rl_moe_select", "rl_moe_plan", "rl_moe_max_tiles", "rl_moe_experts", "rl_embed_pair",
@@ -2053,3 +2058,233 @@ def gated_join_norm(y0, s0: float, y1, s1: float, z, gamma, eps: float, alpha: f
                                    _ptr(z), 0 if z is None else z.stride(0), _ptr(z_bias), _ptr(gamma), _ptr(stream_rows), stream_rows.stride(0), _ptr(copy),
                                    0 if copy is None else copy.stride(0), n, width, float(eps), float(alpha), _stream())
     _ok(rc, "gated_join_norm")
+
+
+# ---- a cache held in 8 bits --------------------------------------------------------------------
+#
+# One layer's cache: ``pool`` float8_e4m3fn [pages, 2 (key, value), kv heads, page size, head dim] and ``scales`` float32 [pages, 2, kv heads,
+# page size / 16].  16 consecutive tokens of a page share one scale a plane and head, a power of two; a value is code * scale.  Page sizes
+# are multiples of 16, head sizes multiples of 32 up to 256.
+
+KV8_BLOCK = 16          # tokens that share a scale
+KV8_TILE_QUERIES = 64   # queries that an entry of a tile list names
+
+
+def kv8_fits(page_size: int, head_dim: int) -> bool:
+    """Whether the kernels of the 8-bit cache take these sizes."""
+    return page_size > 0 and page_size % KV8_BLOCK == 0 and 0 < head_dim <= 256 and head_dim % 32 == 0
+
+
+def _kv8_pool(pool, scales, what: str) -> tuple[int, int, int, int]:
+    """(pages, kv heads, page size, head dim) of a checked 8-bit cache."""
+    if pool.dim() != 5 or pool.shape[1] != 2:
+        raise KernelError(f"{what}: the pool must be [pages, 2, kv heads, page size, head dim]")
+    _need(pool, "pool", torch.float8_e4m3fn)
+    _need(scales, "scales", torch.float32)
+    n_pages, _, n_kv, page_size, dh = pool.shape
+    if not kv8_fits(page_size, dh):
+        raise KernelError(f"{what}: page size {page_size} must be a multiple of {KV8_BLOCK} and head size {dh} one of 32, up to 256")
+    if tuple(scales.shape) != (n_pages, 2, n_kv, page_size // KV8_BLOCK):
+        raise KernelError(f"{what}: scales must be [pages, 2, kv heads, page size / {KV8_BLOCK}]")
+    if pool.data_ptr() % 16:
+        raise KernelError(f"{what}: the pool must begin at a multiple of 16 bytes")
+    return n_pages, n_kv, page_size, dh
+
+
+def _on_current_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """Kernels are launched on the current device's stream: every tensor has to live there."""
+    here = torch.cuda.current_device()
+    for t in (first, *others):
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{here}")
+
+
+def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start, slots, max_pos: int) -> None:
+    """Write the step's keys and values into an 8-bit cache (csrc/kv8_write.cu).
+
+    ``k``, ``v`` [tokens, kv heads * head dim], both float32 or both bfloat16 (views with a row stride, as the columns of a packed
+    product); token t is at position ``positions[t]`` of request ``req_of_token[t]``, whose cache pages are row
+    ``slots[request]`` of ``block_table``; a request's tokens are consecutive, from ``q_start[request]`` on, at consecutive positions, and
+    no two requests share a page that the step writes.  A block of 16 tokens gets the smallest power of two s as its scale with which
+    all that the step brings into it is at most 448 s; a block that holds earlier tokens of the request keeps its scale if that is larger, and
+    where it is not, the earlier codes are brought to the new one.  An infinity or NaN is stored as NaN and does not count for the scale.
+    Nothing else of the cache changes.  A position outside 0 .. max_pos - 1 or a block table without a page sets the status word, and the
+    tokens concerned are not written."""
+    n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_write")
+    _need(k, "k", contiguous=False)
+    _need(v, "v", k.dtype, contiguous=False)
+    code = _code(k)
+    n = positions.numel()
+    for x in (k, v):
+        if x.dim() != 2 or x.shape[0] < n or x.shape[1] != n_kv * dh or x.stride(1) != 1:
+            raise KernelError("kv8_write: k and v must be rows of kv heads * head size entries, one a token")
+        if x.data_ptr() % 16 or (x.stride(0) * x.element_size()) % 16:
+            raise KernelError("kv8_write: rows of k and v must begin at multiples of 16 bytes")
+    for t, name in ((block_table, "block_table"), (positions, "positions"), (req_of_token, "req_of_token"), (q_start, "q_start"), (slots, "slots")):
+        _need(t, name, torch.int32)
+    if block_table.dim() != 2 or req_of_token.numel() < n:
+        raise KernelError("kv8_write: block_table must be [slots, pages], and req_of_token as long as positions")
+    _on_current_device("kv8_write", pool, scales, k, v, block_table, positions, req_of_token, q_start, slots)
+    if n == 0:
+        return
+    rc = _lib().rl_kv8_write(code, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), pool.data_ptr(), scales.data_ptr(),
+                             block_table.data_ptr(), block_table.shape[0], block_table.shape[1], positions.data_ptr(), req_of_token.data_ptr(),
+                             q_start.data_ptr(), slots.data_ptr(), n, q_start.numel() - 1, n_kv, dh, page_size, n_pages, int(max_pos),
+                             status_word(pool.device).data_ptr(), _stream())
+    _ok(rc, "kv8_write")
+
+
+_KV8_PLANS: dict[tuple, tuple[int, int, int, int, int]] = {}
+
+
+def _kv8_plan(n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, span: int) -> tuple[int, int, int, int, int]:
+    """(warps along the rows, blocks of rows, parts of the keys, keys of a part, rows of scratch) for items of up to ``queries`` queries."""
+    key = (n_items, queries, n_heads, n_kv, dh, span)
+    have = _KV8_PLANS.get(key)
+    if have is not None:
+        return have
+    rows = queries * (n_heads // n_kv)
+    wr = 1 if rows <= 16 else 4
+    row_blocks = -(-rows // (16 * wr))
+    units = n_items * n_kv * row_blocks
+    parts = max(1, min(-(-span // 256), 4 * sm_count() // units, 64))
+    chunk = -(-span // (parts * 64)) * 64
+    parts = max(1, -(-span // chunk))
+    scratch = units * parts * 16 * wr if parts > 1 else 0
+    if len(_KV8_PLANS) > 4096:
+        _KV8_PLANS.clear()
+    have = _KV8_PLANS[key] = (wr, row_blocks, parts, chunk, scratch)
+    return have
+
+
+def _kv8_plans(n_tiles: int, max_q: int, n_decode: int, n_heads: int, n_kv: int, dh: int, span: int, window: int):
+    """The plans of a call's portions and of its decoded requests (``None``: there are none)."""
+    queries = min(max(int(max_q), 1), KV8_TILE_QUERIES)
+    if window > 0:
+        span = min(span, window + queries)
+    span = max(span, 1)
+    return (_kv8_plan(n_tiles, queries, n_heads, n_kv, dh, span) if n_tiles else None,
+            _kv8_plan(n_decode, 1, n_heads, n_kv, dh, span) if n_decode else None)
+
+
+def kv8_attention_scratch(*, n_heads: int, n_kv: int, head_dim: int, span: int, n_tiles: int = 0, max_q: int = KV8_TILE_QUERIES,
+                          n_decode: int = 0, window: int | None = None) -> int:
+    """How many floats of scratch ``kv8_attention`` needs for these sizes (0: none)."""
+    plans = _kv8_plans(n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, int(span), int(window or 0))
+    return max((plan[4] * (head_dim + 2) for plan in plans if plan is not None), default=0)
+
+
+def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, n_heads: int, scale: float, span: int,
+                  window: int | None = None, tiles=None, n_tiles: int = 0, max_q: int = KV8_TILE_QUERIES, decode_reqs=None, n_decode: int = 0,
+                  scratch=None) -> None:
+    """Causal attention of the step's queries over an 8-bit cache: ``attention`` with keys and values code * scale
+    (csrc/kv8_attention.cuh).
+
+    ``q`` [tokens, heads * head dim] float32 or bfloat16 (a view with a row stride), ``out`` the same shape and type (rows at multiples of
+    16 bytes).  ``tiles`` int32 [n_tiles, 2]: (request, first query) of every 64 queries of the requests that bring several (``max_q``: the most
+    that one of them brings), ``decode_reqs`` int32 [n_decode]: the requests that bring one.  Rows of ``out`` that belong to
+    neither are left as they are.  A query without a key in sight (``kv_len`` 0, or pages missing, which sets the status word) gets zeros.
+    ``span``: the longest context of these requests; it decides how their keys are cut over blocks, not which keys
+    are seen (a captured call serves longer contexts too).  ``scratch``: float32, ``kv8_attention_scratch`` entries, for the results of
+    parts of the keys; none given, it is allocated for the call (a call that is being recorded has to bring its own).  Calls that may run
+    at the same time need scratch of their own."""
+    n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_attention")
+    _need(q, "q", contiguous=False)
+    _need(out, "out", q.dtype, contiguous=False)
+    code = _code(q)
+    if n_heads <= 0 or n_heads % n_kv != 0:
+        raise KernelError(f"kv8_attention: {n_heads} heads are not a multiple of {n_kv} key/value heads")
+    for x, name in ((q, "q"), (out, "out")):
+        if x.dim() != 2 or x.shape[1] != n_heads * dh or x.stride(1) != 1:
+            raise KernelError(f"kv8_attention: {name} must be rows of heads * head size entries")
+        if x.data_ptr() % 16 or (x.stride(0) * x.element_size()) % 16:
+            raise KernelError(f"kv8_attention: rows of {name} must begin at multiples of 16 bytes")
+    if out.shape[0] < q.shape[0]:
+        raise KernelError("kv8_attention: out has fewer rows than q")
+    for t, name in ((block_table, "block_table"), (q_start, "q_start"), (kv_len, "kv_len"), (slots, "slots")):
+        _need(t, name, torch.int32)
+    if block_table.dim() != 2:
+        raise KernelError("kv8_attention: block_table must be [slots, pages]")
+    if n_tiles > 0:
+        if tiles is None:
+            raise KernelError("kv8_attention: n_tiles without tiles")
+        _need(tiles, "tiles", torch.int32)
+        if tiles.numel() < 2 * n_tiles:
+            raise KernelError("kv8_attention: tiles is shorter than n_tiles")
+    if n_decode > 0:
+        if decode_reqs is None:
+            raise KernelError("kv8_attention: n_decode without decode_reqs")
+        _need(decode_reqs, "decode_reqs", torch.int32)
+        if decode_reqs.numel() < n_decode:
+            raise KernelError("kv8_attention: decode_reqs is shorter than n_decode")
+    if window is not None and window <= 0:
+        raise KernelError("kv8_attention: a window sees at least one key")
+    _on_current_device("kv8_attention", pool, scales, q, out, block_table, q_start, kv_len, slots,
+                       tiles if n_tiles > 0 else None, decode_reqs if n_decode > 0 else None, scratch)
+    if q.shape[0] == 0:
+        return
+    window = int(window or 0)
+    plans = _kv8_plans(n_tiles, max_q, n_decode, n_heads, n_kv, dh, int(span), window)
+    need = max((plan[4] * (dh + 2) for plan in plans if plan is not None), default=0)
+    if need:
+        if scratch is None:
+            if _recorder is not None:
+                raise KernelError("kv8_attention: a recorded call needs scratch that outlives it")
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        _need(scratch, "scratch", torch.float32)
+        if scratch.numel() < need or scratch.data_ptr() % 16:
+            raise KernelError(f"kv8_attention: scratch of {need} floats at a multiple of 16 bytes is needed")
+    lib = _lib()
+    for plan, items, n_items, is_tiles in ((plans[0], tiles, n_tiles, 1), (plans[1], decode_reqs, n_decode, 0)):
+        if plan is None:
+            continue
+        wr, row_blocks, parts, chunk, rows = plan
+        part_o = scratch.data_ptr() if rows else None
+        made = lib.rl_launches_made()
+        rc = lib.rl_kv8_attention(code, q.data_ptr(), q.stride(0), pool.data_ptr(), scales.data_ptr(), block_table.data_ptr(),
+                                  block_table.shape[0], block_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), slots.data_ptr(),
+                                  out.data_ptr(), out.stride(0), items.data_ptr(), n_items, is_tiles, q.shape[0], n_heads, n_kv, dh,
+                                  page_size, n_pages, window, float(scale), wr, row_blocks, parts, chunk, part_o,
+                                  part_o + rows * dh * 4 if rows else None, status_word(q.device).data_ptr(), _stream())
+        _ok(rc, "kv8_attention", made)
+
+
+# ---- copies of cache pages -----------------------------------------------------------------------
+
+class PagePools:
+    """The tensors that hold a cache's pages (first extent: pages, as many in each), for ``copy_pages``: codes, scales or rows of every
+    layer.  The tensors are kept alive."""
+
+    def __init__(self, pools) -> None:
+        self.pools = list(pools)
+        if not self.pools:
+            raise KernelError("PagePools: no pool given")
+        self.n_pages = self.pools[0].shape[0]
+        for t in self.pools:
+            _need(t, "a pool")
+            if t.shape[0] != self.n_pages:
+                raise KernelError("PagePools: the pools have different numbers of pages")
+            if t.device != self.pools[0].device:
+                raise KernelError("PagePools: the pools are on different devices")
+            if self.n_pages and (t.numel() // self.n_pages * t.element_size() % 4 or t.numel() == 0 or t.data_ptr() % 4):
+                raise KernelError("PagePools: a page must be a multiple of 4 bytes, at a multiple of 4 bytes")
+        n = len(self.pools)
+        self.bases = (c_void_p * n)(*(t.data_ptr() for t in self.pools))
+        self.page_bytes = (c_long * n)(*(t.numel() // max(1, self.n_pages) * t.element_size() for t in self.pools))
+
+
+def copy_pages(pools: PagePools, pairs) -> None:
+    """Page ``pairs[i][0]`` to page ``pairs[i][1]`` in every pool, for all i at once (csrc/copy_pages.cu).  ``pairs`` int32 [n, 2] on the
+    device; no page is the target of two pairs, or the target of one and the source of another.  Pages that are not in the pools set the
+    status word and are not copied."""
+    _need(pairs, "pairs", torch.int32)
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise KernelError("copy_pages: pairs must be [n, 2]")
+    _on_current_device("copy_pages", pools.pools[0], pairs)
+    if pairs.shape[0] == 0:
+        return
+    lib = _lib()
+    made = lib.rl_launches_made()
+    rc = lib.rl_copy_pages(pools.bases, pools.page_bytes, len(pools.pools), pairs.data_ptr(), pairs.shape[0], pools.n_pages,
+                           status_word(pairs.device).data_ptr(), _stream())
+    _ok(rc, "copy_pages", made)
