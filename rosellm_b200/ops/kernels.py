@@ -2138,22 +2138,22 @@ _KV8_PLANS: dict[tuple, tuple[int, int, int, int, int]] = {}
 
 
 def _kv8_plan(n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, span: int) -> tuple[int, int, int, int, int]:
-    """(warps along the rows, blocks of rows, parts of the keys, keys of a part, rows of scratch) for items of up to ``queries`` queries."""
+    """(rows of a block of threads, blocks of rows, parts of the keys, keys of a part, rows of scratch) for items of up to ``queries`` queries."""
     key = (n_items, queries, n_heads, n_kv, dh, span)
     have = _KV8_PLANS.get(key)
     if have is not None:
         return have
     rows = queries * (n_heads // n_kv)
-    wr = 1 if rows <= 16 else 4
-    row_blocks = -(-rows // (16 * wr))
+    block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
+    row_blocks = -(-rows // block)
     units = n_items * n_kv * row_blocks
-    parts = max(1, min(-(-span // 256), 4 * sm_count() // units, 64))
+    parts = max(1, min(-(-span // 256), 8 * sm_count() // units, 64))
     chunk = -(-span // (parts * 64)) * 64
     parts = max(1, -(-span // chunk))
-    scratch = units * parts * 16 * wr if parts > 1 else 0
+    scratch = units * parts * block if parts > 1 else 0
     if len(_KV8_PLANS) > 4096:
         _KV8_PLANS.clear()
-    have = _KV8_PLANS[key] = (wr, row_blocks, parts, chunk, scratch)
+    have = _KV8_PLANS[key] = (block, row_blocks, parts, chunk, scratch)
     return have
 
 
@@ -2238,13 +2238,13 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     for plan, items, n_items, is_tiles in ((plans[0], tiles, n_tiles, 1), (plans[1], decode_reqs, n_decode, 0)):
         if plan is None:
             continue
-        wr, row_blocks, parts, chunk, rows = plan
+        block, row_blocks, parts, chunk, rows = plan
         part_o = scratch.data_ptr() if rows else None
         made = lib.rl_launches_made()
         rc = lib.rl_kv8_attention(code, q.data_ptr(), q.stride(0), pool.data_ptr(), scales.data_ptr(), block_table.data_ptr(),
                                   block_table.shape[0], block_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), slots.data_ptr(),
                                   out.data_ptr(), out.stride(0), items.data_ptr(), n_items, is_tiles, q.shape[0], n_heads, n_kv, dh,
-                                  page_size, n_pages, window, float(scale), wr, row_blocks, parts, chunk, part_o,
+                                  page_size, n_pages, window, float(scale), block, row_blocks, parts, chunk, part_o,
                                   part_o + rows * dh * 4 if rows else None, status_word(q.device).data_ptr(), _stream())
         _ok(rc, "kv8_attention", made)
 
