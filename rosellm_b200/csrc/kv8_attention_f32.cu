@@ -3,6 +3,8 @@
 
 namespace rl {
 namespace kv8 {
-int attention8_f32(const AttnParams8& p, int n_items, int rows, cudaStream_t stream) { return dispatch_attention8<true>(p, n_items, rows, stream); }
+int attention8_f32(const AttnParams8& p, int rows, int blocks, Fit* fit, cudaStream_t stream) {
+  return dispatch_attention8<true>(p, rows, blocks, fit, stream);
+}
 }  // namespace kv8
 }  // namespace rl

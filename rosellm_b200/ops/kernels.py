@@ -122,7 +122,8 @@ class _RecordingLib:
 _NOT_KERNELS = ("rl_copy_to_device", "rl_event_record")  # library functions that put something else on the stream
 _QUERIES = ("rl_gemm_tc_rows_fits", "rl_gemm_rows_smem_fits", "rl_mlp_fused_slice", "rl_attn_block_fused_fits", "rl_attn_block_fused_cluster",
             "rl_host_memory_on_device", "rl_latent_attention_fits", "rl_latent_decode_fits",
-            "rl_launches_made", "rl_gemm_rows_ring_fits", "rl_gemm_tile_f32_for", "rl_moe_max_tiles", "rl_bias_attention_shape", "rl_recurrence_record", "rl_rmsnorm_add_experts_fits")  # library functions that launch nothing
+            "rl_launches_made", "rl_gemm_rows_ring_fits", "rl_gemm_tile_f32_for", "rl_moe_max_tiles", "rl_bias_attention_shape", "rl_recurrence_record", "rl_rmsnorm_add_experts_fits",
+            "rl_kv8_attention_blocks")  # library functions that launch nothing
 
 
 class recording:
@@ -232,9 +233,10 @@ def _lib() -> ctypes.CDLL:
         lib.rl_gated_join_norm.argtypes = [P, L, F, P, L, F, P, L, P, P, P, L, P, L, I, I, F, F, P]
         lib.rl_bias_kv_store.argtypes = [I, P, L, P, L, P, P, I, P, P, L, P, P, P, I, I, I, I, I, I, I, I, P, P]
         lib.rl_kv8_write.argtypes = [I, P, L, P, L, P, P, P, I, I, P, P, P, P, I, I, I, I, I, I, I, P, P]
-        lib.rl_kv8_attention.argtypes = [I, P, L, P, P, P, I, I, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, P, P, P, P]
+        lib.rl_kv8_attention.argtypes = [I, P, L, P, P, P, I, I, P, P, P, P, L, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, P, P, P, P, P]
+        lib.rl_kv8_attention_blocks.argtypes = [I, I, I, I, I, I]
         lib.rl_copy_pages.argtypes = [P, P, I, P, I, I, P, P]
-        for name in ("rl_kv8_write", "rl_kv8_attention", "rl_copy_pages"):
+        for name in ("rl_kv8_write", "rl_kv8_attention", "rl_kv8_attention_blocks", "rl_copy_pages"):
             getattr(lib, name).restype = I
         for name in ("rl_rmsnorm", "rl_rmsnorm_add", "rl_cast_rows", "rl_latent_attention_fits", "rl_latent_decode_fits",
                      "rl_latent_kv_write", "rl_latent_q_rope", "rl_latent_attention", "rl_head_linear", "rl_gated_act",
@@ -2134,44 +2136,61 @@ def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start,
     _ok(rc, "kv8_write")
 
 
-_KV8_PLANS: dict[tuple, tuple[int, int, int, int, int]] = {}
+_KV8_PLANS: dict[tuple, tuple[int, int, int, int, int, int]] = {}
 
 
-def _kv8_plan(n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, span: int) -> tuple[int, int, int, int, int]:
-    """(rows of a block of threads, blocks of rows, parts of the keys, keys of a part, rows of scratch) for items of up to ``queries`` queries."""
-    key = (n_items, queries, n_heads, n_kv, dh, span)
+def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, span: int) -> tuple[int, int, int, int, int, int]:
+    """(rows of a block of threads, blocks of rows, SMs or 0, blocks of threads, ints of the plan, floats of scratch) for items of up to
+    ``queries`` queries.
+
+    SMs 0: every unit (an item's rows for one key/value head) has a block to itself; else all keys are shared evenly by as many blocks as stand on
+    the device at once, and what lies in several is joined."""
+    key = (code, is_tiles, n_items, queries, n_heads, n_kv, dh, span)
     have = _KV8_PLANS.get(key)
     if have is not None:
         return have
     rows = queries * (n_heads // n_kv)
     block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
     row_blocks = -(-rows // block)
-    units = n_items * n_kv * row_blocks
-    parts = max(1, min(-(-span // 256), 8 * sm_count() // units, 64))
-    chunk = -(-span // (parts * 64)) * 64
-    parts = max(1, -(-span // chunk))
-    scratch = units * parts * block if parts > 1 else 0
+    entries = n_items * row_blocks
+    sms = sm_count()
+    at_once = sms * _lib().rl_kv8_attention_blocks(code, block, is_tiles, n_heads, n_kv, dh)
+    if _kv8_by_units(dh, span) or entries > KV8_MOST_ENTRIES:
+        have = (block, row_blocks, 0, 0, 0, 0)
+    else:
+        plan = -(-(entries + 2) // 4) * 4
+        have = (block, row_blocks, sms, at_once, plan, plan + at_once * 2 * block * (dh + 2))
     if len(_KV8_PLANS) > 4096:
         _KV8_PLANS.clear()
-    have = _KV8_PLANS[key] = (block, row_blocks, parts, chunk, scratch)
+    _KV8_PLANS[key] = have
     return have
 
 
-def _kv8_plans(n_tiles: int, max_q: int, n_decode: int, n_heads: int, n_kv: int, dh: int, span: int, window: int):
+KV8_MOST_ENTRIES = 4096  # blocks of rows whose keys are shared evenly: their numbers lie in shared memory once
+
+
+def _kv8_by_units(dh: int, span: int) -> bool:
+    """Whether units are short enough for a block each: up to 256 KB of keys and values.  Measured on B200, us, by units / shared evenly: 12 heads of
+    64, one request of 700 keys 8.7 / 11.8, 16 of up to 1024 11.8 / 16.9, 32 of 512 9.1 / 17.2, 25 heads, 64 of 1023 38.8 / 40.1; 16 heads, 4 of 2048
+    15.5 / 15.1.  8 heads of 128, 256 of 1024 71.1 / 69.8, 16 of 2048 28.5 / 23.3, 64 of 2048 57.9 / 37.0, 32 of 16384 221 / 100."""
+    return span * 2 * dh <= 256 << 10
+
+
+def _kv8_plans(code: int, n_tiles: int, max_q: int, n_decode: int, n_heads: int, n_kv: int, dh: int, span: int, window: int):
     """The plans of a call's portions and of its decoded requests (``None``: there are none)."""
     queries = min(max(int(max_q), 1), KV8_TILE_QUERIES)
     if window > 0:
         span = min(span, window + queries)
     span = max(span, 1)
-    return (_kv8_plan(n_tiles, queries, n_heads, n_kv, dh, span) if n_tiles else None,
-            _kv8_plan(n_decode, 1, n_heads, n_kv, dh, span) if n_decode else None)
+    return (_kv8_plan(code, 1, n_tiles, queries, n_heads, n_kv, dh, span) if n_tiles else None,
+            _kv8_plan(code, 0, n_decode, 1, n_heads, n_kv, dh, span) if n_decode else None)
 
 
-def kv8_attention_scratch(*, n_heads: int, n_kv: int, head_dim: int, span: int, n_tiles: int = 0, max_q: int = KV8_TILE_QUERIES,
-                          n_decode: int = 0, window: int | None = None) -> int:
+def kv8_attention_scratch(*, dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, span: int, n_tiles: int = 0,
+                          max_q: int = KV8_TILE_QUERIES, n_decode: int = 0, window: int | None = None) -> int:
     """How many floats of scratch ``kv8_attention`` needs for these sizes (0: none)."""
-    plans = _kv8_plans(n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, int(span), int(window or 0))
-    return max((plan[4] * (head_dim + 2) for plan in plans if plan is not None), default=0)
+    plans = _kv8_plans(F32 if dtype == torch.float32 else BF16, n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, int(span), int(window or 0))
+    return max((plan[5] for plan in plans if plan is not None), default=0)
 
 
 def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, n_heads: int, scale: float, span: int,
@@ -2184,9 +2203,9 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     16 bytes).  ``tiles`` int32 [n_tiles, 2]: (request, first query) of every 64 queries of the requests that bring several (``max_q``: the most
     that one of them brings), ``decode_reqs`` int32 [n_decode]: the requests that bring one.  Rows of ``out`` that belong to
     neither are left as they are.  A query without a key in sight (``kv_len`` 0, or pages missing, which sets the status word) gets zeros.
-    ``span``: the longest context of these requests; it decides how their keys are cut over blocks, not which keys
-    are seen (a captured call serves longer contexts too).  ``scratch``: float32, ``kv8_attention_scratch`` entries, for the results of
-    parts of the keys; none given, it is allocated for the call (a call that is being recorded has to bring its own).  Calls that may run
+    ``span``: the longest context of these requests; it decides how their keys are shared out over blocks, not which keys
+    are seen (a captured call serves longer contexts too).  ``scratch``: float32, ``kv8_attention_scratch`` entries, for results of
+    shares of the keys; none given, it is allocated for the call (a call that is being recorded has to bring its own).  Calls that may run
     at the same time need scratch of their own."""
     n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_attention")
     _need(q, "q", contiguous=False)
@@ -2224,8 +2243,8 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     if q.shape[0] == 0:
         return
     window = int(window or 0)
-    plans = _kv8_plans(n_tiles, max_q, n_decode, n_heads, n_kv, dh, int(span), window)
-    need = max((plan[4] * (dh + 2) for plan in plans if plan is not None), default=0)
+    plans = _kv8_plans(code, n_tiles, max_q, n_decode, n_heads, n_kv, dh, int(span), window)
+    need = max((plan[5] for plan in plans if plan is not None), default=0)
     if need:
         if scratch is None:
             if _recorder is not None:
@@ -2238,14 +2257,14 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     for plan, items, n_items, is_tiles in ((plans[0], tiles, n_tiles, 1), (plans[1], decode_reqs, n_decode, 0)):
         if plan is None:
             continue
-        block, row_blocks, parts, chunk, rows = plan
-        part_o = scratch.data_ptr() if rows else None
+        block, row_blocks, sms, at_once, ints, _ = plan
+        at = scratch.data_ptr() if sms else 0
         made = lib.rl_launches_made()
         rc = lib.rl_kv8_attention(code, q.data_ptr(), q.stride(0), pool.data_ptr(), scales.data_ptr(), block_table.data_ptr(),
                                   block_table.shape[0], block_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), slots.data_ptr(),
                                   out.data_ptr(), out.stride(0), items.data_ptr(), n_items, is_tiles, q.shape[0], n_heads, n_kv, dh,
-                                  page_size, n_pages, window, float(scale), block, row_blocks, parts, chunk, part_o,
-                                  part_o + rows * dh * 4 if rows else None, status_word(q.device).data_ptr(), _stream())
+                                  page_size, n_pages, window, float(scale), block, row_blocks, sms, at_once, at, at + 4 * ints,
+                                  at + 4 * (ints + at_once * 2 * block * dh), status_word(q.device).data_ptr(), _stream())
         _ok(rc, "kv8_attention", made)
 
 

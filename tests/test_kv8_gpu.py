@@ -286,7 +286,7 @@ def test_no_key_in_sight(K, dtype):
 def test_captured_and_longer(K):
     """A graph captured at one length serves longer ones, and its own scratch, on a stream of its own."""
     page, heads = 16, 4
-    batch = P.Batch([(2000, 1), (700, 1), (1900, 6)], page)
+    batch = P.Batch([(5000, 1), (700, 1), (3900, 6)], page)
     gen = torch.Generator().manual_seed(5)
     pool, scales = cache_of(batch, heads, 64, gen)
     pool, scales = pool.to(DEV), scales.to(DEV)
@@ -296,18 +296,18 @@ def test_captured_and_longer(K):
     out = torch.zeros(batch.tokens, heads * 64, dtype=BF16, device=DEV)
 
     def go(into):
-        K.kv8_attention(q, pool, scales, a["block_table"], a["q_start"], a["kv_len"], a["slots"], into, n_heads=heads, scale=0.125, span=900,
+        K.kv8_attention(q, pool, scales, a["block_table"], a["q_start"], a["kv_len"], a["slots"], into, n_heads=heads, scale=0.125, span=2100,
                         tiles=a["tiles"], n_tiles=1, max_q=6, decode_reqs=a["decode_reqs"], n_decode=2)
 
-    assert K.kv8_attention_scratch(n_heads=heads, n_kv=heads, head_dim=64, span=900, n_tiles=1, max_q=6, n_decode=2) > 0
-    a["kv_len"].copy_(torch.tensor([900, 30, 600], dtype=torch.int32))
+    assert K.kv8_attention_scratch(dtype=BF16, n_heads=heads, n_kv=heads, head_dim=64, span=2100, n_tiles=1, max_q=6, n_decode=2) > 0
+    a["kv_len"].copy_(torch.tensor([2100, 30, 600], dtype=torch.int32))
     go(out)
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
         go(out)
-    for lens in (full, torch.tensor([900, 30, 600], dtype=torch.int32, device=DEV), torch.tensor([1, 1, 6], dtype=torch.int32, device=DEV)):
+    for lens in (full, torch.tensor([2100, 30, 600], dtype=torch.int32, device=DEV), torch.tensor([1, 1, 6], dtype=torch.int32, device=DEV)):
         a["kv_len"].copy_(lens)
         graph.replay()
         torch.cuda.synchronize()
