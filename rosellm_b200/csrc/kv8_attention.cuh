@@ -47,8 +47,9 @@ struct AttnParams8 {
   int row_blocks;      // blocks of rows of an item and key/value head
   int n_entries;       // items * row_blocks
   int balanced;        // 0: a unit (an entry's rows for one key/value head) a block; else all tiles of all units in equal runs
-  int* plan;           // balanced: a run's length, then what the entries before each entry come to for one head [n_entries + 1]
-  float* part_o;       // balanced: [blocks][2][rows][head dim], results of units that a run has not the whole of
+  int cost;            // balanced: what beginning a unit counts for, in tiles
+  int* plan;           // a run's length, then what the entries before each entry come to for one head [n_entries + 1]
+  float* part_o;       // [blocks][2][rows][head dim], results of units that a run has not the whole of
   float* part_ml;      // [blocks][2][rows][2]
   int ring, region;    // tiles that the ring holds; bytes of one warp's outputs on their way to another
   int* status;
@@ -224,8 +225,6 @@ struct Queries {
     }
   }
 };
-
-constexpr int COST = 8;  // what beginning a unit costs a block, in tiles: about 2 us
 
 constexpr float NOTHING = -1.7e38f;  // the maximum of no score: finite, so that differences are never of two infinities
 
@@ -513,7 +512,7 @@ __device__ __forceinline__ bool read_answer(uint32_t answer, int& x, int& y) {
 // fetching warp is by then ahead in that one's keys: a block of short contexts ends long before its loads have been worth their latency.
 //
 // 1: the tiles of all units in a row, and in front of each unit's the cost of beginning one, are cut into as many equal runs as blocks stand on the device
-// at once (but runs of at least COST + 4 tiles, or of up to COST + 16 where there is one for each SM), whatever the lengths.  A unit that a
+// at once (but runs of at least p.cost + 4 tiles, or of up to p.cost + 16 where there is one for each SM), whatever the lengths.  A unit that a
 // run has the whole of goes to the output; of others, a run has at most two, and kv8_join_kernel joins their parts.  32 contexts of up to 16384 tokens, 8 heads of 128: 114 us in parts of 1536
 // keys that blocks take over from one another, which leaves the last of them waiting for the longest.
 //
@@ -554,7 +553,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
   if (p.balanced) {
     for (int e = threadIdx.x; e < p.n_entries; e += 160) {
       const int tiles = work_of<L::RB>(p, e).tiles(TB);
-      before[e] = tiles > 0 ? COST + tiles : 0;
+      before[e] = tiles > 0 ? p.cost + tiles : 0;
     }
     __syncthreads();
     if (warp == 0) {
@@ -670,7 +669,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
 
     if (p.balanced) {
       const int total = before[p.n_entries] * p.n_kv_heads, blocks = (int)gridDim.x;
-      const int run = max((total + blocks - 1) / blocks, min(max((total + p.balanced - 1) / p.balanced, COST + 4), COST + 16));
+      const int run = max((total + blocks - 1) / blocks, min(max((total + p.balanced - 1) / p.balanced, p.cost + 4), p.cost + 16));
       if (blockIdx.x == 0) {  // for the kernel that joins
         for (int e = lane; e <= p.n_entries; e += 32) p.plan[1 + e] = before[e];
         if (lane == 0) p.plan[0] = run;
@@ -691,11 +690,11 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
         const Work w = work_of<L::RB>(p, entry);
         const int tiles = w.tiles(TB);
         if (tiles == 0) continue;
-        int h = rest / (COST + tiles), off = rest - h * (COST + tiles);
+        int h = rest / (p.cost + tiles), off = rest - h * (p.cost + tiles);
         rest = 0;
         for (; h < p.n_kv_heads && at < end && ok; ++h) {
-          const int n = min(COST + tiles - off, end - at), i0 = max(off - COST, 0), i1 = max(off + n - COST, 0);
-          if (i1 > i0) serve(w, h, i0, i1, i1 - i0 == tiles ? -1 : (int)blockIdx.x * 2 + (off >= COST ? 0 : 1));
+          const int n = min(p.cost + tiles - off, end - at), i0 = max(off - p.cost, 0), i1 = max(off + n - p.cost, 0);
+          if (i1 > i0) serve(w, h, i0, i1, i1 - i0 == tiles ? -1 : (int)blockIdx.x * 2 + (off >= p.cost ? 0 : 1));
           at += n;
           off = 0;
         }
@@ -915,7 +914,7 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   pdl_begin();
   const int run = p.plan[0], mine = p.plan[1 + blockIdx.x], cost = p.plan[2 + blockIdx.x] - mine;
   if (cost <= 0) return;
-  const int begin = mine * p.n_kv_heads + blockIdx.y * cost + COST, first = begin / run, parts = (begin + cost - COST - 1) / run - first + 1;
+  const int begin = mine * p.n_kv_heads + blockIdx.y * cost + p.cost, first = begin / run, parts = (begin + cost - p.cost - 1) / run - first + 1;
   if (parts <= 1) return;
   const Work w = work_of<RB>(p, blockIdx.x);
   const Rows rows{w.token0, w.pos0, w.first_row, w.rows, (int)blockIdx.y};
@@ -978,6 +977,7 @@ int launch_attention(AttnParams8 p, int most_rows, int blocks, Fit* fit, cudaStr
   }
   p.ring = f.ring;
   p.region = f.region;
+  p.cost = 8;  // about 2 us
   if (p.balanced && (p.n_entries + 1) * 4 > f.ring * L::SLOT) return -10;  // the ring's place holds the entries' tiles at first
   const auto kernel = kv8_attention_kernel<DH, F32, NR, WR>;
   const int rc = (int)note_launch(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f.bytes));

@@ -1,0 +1,686 @@
+// Attention over the 8-bit cache on tcgen05, for many rows (bfloat16, head sizes 64 and 128): the function of kv8_attention.cuh.
+//
+// A block of threads takes 128 rows, queries times the heads that share one key/value head, and walks their keys in tiles of 128.  Its warps:
+//   0-3    bring codes from memory to registers, a tile ahead, turn them into halves (exact) and write those into the swizzled layouts that the
+//          products read, keys and values apart, two stages of each;
+//   4-11   softmax, two groups of four warps on alternate tiles, a thread a row: read the scores from tensor memory, write the
+//          probabilities back over them as halves.  Each group has a maximum, a sum and an output of its own; they meet at the end of the unit;
+//   12     issues S = Q K^T (M 128, N 128) and O += P V (P taken from tensor memory, V as it lies);
+//   13     says which tiles of which unit come next.
+// Tensor memory: two tiles of scores, 128 columns each, and two outputs of head dim columns.
+//
+// Scales as in kv8_attention.cuh: a block of 16 keys is 16 columns of the scores, so a key scale is a factor of 16 columns' exponents and a value
+// scale one of their probabilities.  The output stays in tensor memory and is multiplied only when a row's maximum has grown by more
+// than 2^8 since it was last (probabilities are at most 2^8 then) or a value scale exceeds the reference; probabilities times share are at
+// most 2^15 and keep 11 bits down to 2^-14.
+//
+// What bounds it: 128 x 128 exponentials take 1024 cycles of an SM, the products of a tile 1024 (head 128) or 512; turning 32 KB of codes into
+// halves takes 260 issue slots a scheduler.  Work is shared over the SMs in equal runs of tiles, as there.
+#pragma once
+#include "kv8_attention.cuh"
+
+namespace rl {
+namespace kv8 {
+
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_BLOCKS = TC_KEYS / BLOCK, TC_THREADS = 448;
+
+template <int DH>
+struct TcLayout {
+  static constexpr int SUBS = DH / 64;                 // stretches of 64 entries, 128 bytes of halves: a row of the swizzle
+  static constexpr int SUB_BYTES = 128 * 128;          // 128 rows of one
+  static constexpr int MAT = SUBS * SUB_BYTES;
+  static constexpr int Q = 0, K = MAT, V = K + 2 * MAT;
+  static constexpr int NAN_BITS = V + 2 * MAT;         // [stage][key][DH / 16] a bit for each value of a tile that not every row sees whole: NaN
+  static constexpr int NAN_SOME = NAN_BITS + 2 * TC_KEYS * (DH / 8);  // [stage][4 warps]: whether there is one
+  static constexpr int ML = NAN_SOME + 2 * 4 * 4;      // [group][128 rows] maximum, sum, reference, whether there is anything
+  static constexpr int FACTOR = ML + 2 * 128 * 16;     // [128 rows]
+  static constexpr int SEG = FACTOR + 512;             // two segments
+  static constexpr int BARS = SEG + 2 * 64;
+  static constexpr int BYTES = BARS + 8 * 24 + 16 + 1024;  // and room to align
+};
+
+enum TcBar { SEG_FULL = 0, SEG_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY = 10, S_FULL = 12, P_READY = 14, PV_DONE = 16, Q_READY = 18, O_FREE = 19, TC_BARS = 20 };
+
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// half x half -> float32, M 128; b_mn: B has its N dimension contiguous
+__host__ __device__ constexpr uint32_t tc_instr_desc(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// An MN-major tile, 128-byte swizzle: rows of 64 entries, groups of eight rows 1024 bytes apart, the next 64 columns a stretch of 128 rows on.
+__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+               "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// Two float32 values as one register pair, for the instructions that take two at a time.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) { return (uint64_t)__float_as_uint(lo) | ((uint64_t)__float_as_uint(hi) << 32); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// What the planning warp tells the others.
+struct TcSegment {
+  int n_tiles;  // -1: no more
+  int key0;     // the first tile's first key
+  int part;     // as in Segment
+  int token0, pos0, first_row, rows, head_kv;
+  int slot, first_seen, end_block;  // the block table's row; blocks of 16 keys from first_seen to end_block - 1 are wanted
+  int pos_lo, pos_hi;               // positions of the first and the last row
+  int pad[3];
+};
+
+template <int DH>
+__global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const AttnParams8 p) {
+  using L = TcLayout<DH>;
+  extern __shared__ uint8_t tc_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)tc_smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t base = tc::smem_u32(smem);
+  auto bar = [&](int which) { return base + L::BARS + 8 * (uint32_t)which; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BARS + 8 * 24);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  TcSegment* segments = reinterpret_cast<TcSegment*>(smem + L::SEG);
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(bar(SEG_FULL + i), 1);
+      tc::mbar_init(bar(SEG_EMPTY + i), 13);
+      tc::mbar_init(bar(K_FULL + i), 4);
+      tc::mbar_init(bar(K_EMPTY + i), 1);
+      tc::mbar_init(bar(V_FULL + i), 4);
+      tc::mbar_init(bar(V_EMPTY + i), 1);
+      tc::mbar_init(bar(S_FULL + i), 1);
+      tc::mbar_init(bar(P_READY + i), 4);
+      tc::mbar_init(bar(PV_DONE + i), 1);
+    }
+    tc::mbar_init(bar(Q_READY), 8);
+    tc::mbar_init(bar(O_FREE), 8);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_begin();
+  // what the entries before each come to for one head, in the place of the first keys
+  int* before = reinterpret_cast<int*>(smem + L::K);
+  for (int e = threadIdx.x; e < p.n_entries; e += TC_THREADS) {
+    const int tiles = work_of<TC_ROWS>(p, e).tiles(TC_BLOCKS);
+    before[e] = tiles > 0 ? p.cost + tiles : 0;
+  }
+  __syncthreads();
+  if (warp == 13) {
+    int sum = 0;
+    for (int e = 0; e < p.n_entries; e += 32) {
+      int x = e + lane < p.n_entries ? before[e + lane] : 0;
+      const int own = x;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (e + lane < p.n_entries) before[e + lane] = sum + x - own;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    __syncwarp();
+    if (lane == 0) before[p.n_entries] = sum;
+    __syncwarp();
+  }
+  // the run of this block, before the numbers' place is written over
+  int at = 0, end = 0, entry = 0, rest = 0;
+  if (warp == 13) {
+    const int total = before[p.n_entries] * p.n_kv_heads, blocks = (int)gridDim.x;
+    const int run = max((total + blocks - 1) / blocks, p.cost + 1);
+    if (blockIdx.x == 0) {  // for the kernel that joins
+      for (int e = lane; e <= p.n_entries; e += 32) p.plan[1 + e] = before[e];
+      if (lane == 0) p.plan[0] = run;
+    }
+    at = blockIdx.x * run;
+    end = min(total, at + run);
+    for (int hi = p.n_entries; hi - entry > 1;) {  // the last entry that begins at or before `at`
+      const int mid = (entry + hi) >> 1;
+      if (before[mid] * p.n_kv_heads <= at)
+        entry = mid;
+      else
+        hi = mid;
+    }
+    rest = at - before[entry] * p.n_kv_heads;
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int group = p.n_heads / p.n_kv_heads, page_blocks = p.page_size / BLOCK;
+  auto wait = [&](int which, uint32_t parity) { return tc::mbar_wait_warp(bar(which), parity, abort_flag, p.status); };
+  // The segment at hand, for the roles below; false when there is none.
+  auto next_segment = [&](uint32_t n, TcSegment& s) {
+    if (!wait(SEG_FULL + (int)(n & 1u), (n >> 1) & 1u)) return false;
+    const int4* from = reinterpret_cast<const int4*>(segments + (n & 1u));
+    const int4 a = from[0], b = from[1], c = from[2];
+    s = TcSegment{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w, from[3].x, {}};
+    return s.n_tiles >= 0;
+  };
+  auto done_with = [&](uint32_t n) {
+    __syncwarp();
+    if (lane == 0) arrive(bar(SEG_EMPTY + (int)(n & 1u)));
+  };
+  auto page_of = [&](const TcSegment& s, int b) {  // of block b; -1: none, -2: not wanted
+    if (b < s.first_seen || b >= s.end_block) return -2;
+    const int e = b / page_blocks;
+    return s.slot >= 0 && s.slot < p.bt_rows && e < p.bt_cols ? p.block_table[(size_t)s.slot * p.bt_cols + e] : -1;
+  };
+  // whether every row of the block of threads sees every key of a tile
+  auto is_whole = [&](const TcSegment& s, int key0) {
+    return key0 + TC_KEYS - 1 <= s.pos_lo && (p.window <= 0 || key0 > s.pos_hi - p.window) && key0 >= s.first_seen * BLOCK;
+  };
+
+  if (warp < 4) {
+    // ---- codes to halves ----
+    constexpr int PIECES = DH / 16;                    // of 16 codes, a thread, of the keys of a tile
+    constexpr int APART = 128 / DH;                    // blocks of 16 keys between two of a thread's pieces
+    const int t = threadIdx.x, own_block = t / DH, key_in_block = t % DH / (DH / 16), part = t % (DH / 16);
+    const size_t to_values = (size_t)p.n_kv_heads * p.page_size * DH;
+    const int in_block = key_in_block * DH + part * 16;
+    // where the piece's halves go: a row of 128 bytes a key, 16-byte pieces swizzled by the key (key % 8 is that of key_in_block)
+    const uint32_t own_row = (uint32_t)(part / 4) * L::SUB_BYTES + (uint32_t)(own_block * BLOCK + key_in_block) * 128u;
+    const uint32_t own_chunk = (uint32_t)((part % 4 * 2) ^ (key_in_block & 7)) << 4;
+    uint4 keys[PIECES], values[PIECES];                // loaded, to be converted next
+    uint32_t count = 0;
+    TcSegment s;
+    bool ok = true;
+    for (uint32_t n = 0; ok && next_segment(n, s); ++n) {
+      // lanes look after a tile's eight blocks (lane % 8): the table's entry, and from it where the block's keys lie (of a block that is not there,
+      // the pool's first: what is read is hidden from every row, and its values are looked through for NaN)
+      auto look_up = [&](int i) { return i < s.n_tiles ? page_of(s, s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7)) : -2; };
+      auto place_of = [&](int page, int i) -> const uint8_t* {
+        if (page != -2 && (page < 0 || page >= p.n_pages)) {
+          atomicOr(p.status, RL_STATUS_BAD_PAGE);
+          page = -1;
+        }
+        const int b = s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7);
+        return page < 0 ? p.pool : p.pool + (((size_t)page * 2 * p.n_kv_heads + s.head_kv) * p.page_size + b % page_blocks * BLOCK) * DH;
+      };
+      auto load = [&](uint4(&to)[PIECES], const uint8_t* place, size_t plane) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const uint8_t* from = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), own_block + APART * j));
+          to[j] = __ldcg(reinterpret_cast<const uint4*>(from + plane + in_block));
+        }
+      };
+      // 16 codes as two 16-byte pieces of a row of halves
+      auto store = [&](uint32_t mat, int j, const uint4& codes) {
+        const uint32_t to = mat + own_row + (uint32_t)j * (APART * BLOCK * 128);
+        const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (h ? own_chunk ^ 16u : own_chunk)), "r"(decode2((uint16_t)w[2 * h])),
+                       "r"(decode2((uint16_t)(w[2 * h] >> 16))), "r"(decode2((uint16_t)w[2 * h + 1])), "r"(decode2((uint16_t)(w[2 * h + 1] >> 16)))
+                       : "memory");
+      };
+      auto tell = [&](int which) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(bar(which));
+      };
+      auto convert_keys = [&](uint4(&from)[PIECES], int i) {
+        const uint32_t of = count + (uint32_t)i, stage = of & 1u;
+        ok = ok && wait(K_EMPTY + (int)stage, ((of >> 1) & 1u) ^ 1u);
+        if (!ok) return;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) store(base + L::K + stage * L::MAT, j, from[j]);
+        tell(K_FULL + (int)stage);
+      };
+      auto convert_values = [&](uint4(&from)[PIECES], int i, bool there) {
+        const uint32_t of = count + (uint32_t)i, stage = of & 1u;
+        ok = ok && wait(V_EMPTY + (int)stage, ((of >> 1) & 1u) ^ 1u);
+        if (!ok) return;
+        if (!there || !is_whole(s, s.key0 + i * TC_KEYS)) {
+          // Values that are NaN must not reach rows that do not see them (0 * NaN is NaN): taken out, and noted for the rows that do.
+          uint16_t* bits = reinterpret_cast<uint16_t*>(smem + L::NAN_BITS) + stage * (TC_KEYS * (DH / 16));
+          uint32_t some = 0;
+#pragma unroll
+          for (int j = 0; j < PIECES; ++j) {
+            uint32_t w[4] = {from[j].x, from[j].y, from[j].z, from[j].w}, found = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t bad = __vcmpeq4(w[k] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              w[k] &= ~bad;
+              found |= (((bad & 0x08040201u) * 0x01010101u) >> 24) << (4 * k);  // a bit a byte
+            }
+            from[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            bits[((own_block + APART * j) * BLOCK + key_in_block) * (DH / 16) + part] = (uint16_t)found;
+            some |= found;
+          }
+          const bool any = __any_sync(0xffffffffu, some != 0u);
+          if (lane == 0) reinterpret_cast<int*>(smem + L::NAN_SOME)[stage * 4 + warp] = any;
+        }
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) store(base + L::V + stage * L::MAT, j, from[j]);
+        tell(V_FULL + (int)stage);
+      };
+      // Keys go two tiles ahead of values: scores of tile i + 2 are asked for when the product of tile i's probabilities ends, and that end is what the
+      // values of tile i + 2 wait for.  What was converted makes room for the next tile's load; table entries are looked up one more ahead.
+      auto all_there = [&](int page) { return __all_sync(0xffffffffu, page >= 0 && page < p.n_pages); };
+      const int e0 = look_up(0), e1 = look_up(1), e2 = look_up(2);
+      int entry_ahead = look_up(3);
+      // places of the values of the next tiles: keys are three tiles ahead when they are loaded
+      const uint8_t *v0 = place_of(e0, 0), *v1 = place_of(e1, 1), *v2 = place_of(e2, 2);
+      bool t0 = all_there(e0), t1 = all_there(e1), t2 = all_there(e2);
+      load(keys, v0, 0);
+      load(values, v0, to_values);
+      convert_keys(keys, 0);
+      load(keys, v1, 0);
+      if (s.n_tiles > 1) convert_keys(keys, 1);
+      load(keys, v2, 0);
+#pragma unroll 1
+      for (int i = 0; i < s.n_tiles && ok; ++i) {
+        convert_values(values, i, t0);
+        load(values, v1, to_values);
+        if (i + 2 < s.n_tiles) convert_keys(keys, i + 2);
+        const uint8_t* v3 = place_of(entry_ahead, i + 3);
+        load(keys, v3, 0);
+        v1 = v2, v2 = v3;
+        t0 = t1, t1 = t2, t2 = all_there(entry_ahead);
+        entry_ahead = look_up(i + 4);
+      }
+      count += (uint32_t)s.n_tiles;
+      done_with(n);
+    }
+  } else if (warp < 12) {
+    // ---- softmax ----
+    const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_at = tmem + lanes + (uint32_t)g * 128u, o_at = tmem + lanes + 256u;
+    auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    auto all_of_us = [&](bool mine) {
+      uint32_t all;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"((uint32_t)mine) : "memory");
+      return all != 0;
+    };
+    float4* ml = reinterpret_cast<float4*>(smem + L::ML);
+    float* factors = reinterpret_cast<float*>(smem + L::FACTOR);
+    uint32_t s_count = 0, pv_count = 0, v_count = 0;  // of this group's tiles; of all tiles (stages go by them)
+    TcSegment s;
+    bool ok = true;
+    for (uint32_t n = 0;; ++n) {
+      const bool have = ok && next_segment(n, s);
+      if (!all_of_us(have)) break;
+      const bool row_ok = row < s.rows, some_row = quarter * 32 < s.rows;
+      const int i_row = s.first_row + min(row, s.rows - 1), q = i_row / group, h = s.head_kv * group + i_row - q * group;
+      const int qpos = s.pos0 + q;
+      float factor = 0.f;
+      if (g == 0) {  // this row's queries as halves, by a power of two that puts the largest entry between 2^14 and 2^15
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)(s.token0 + q) * p.q_stride + (size_t)h * DH);
+        float top = 0.f;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 126);
+          const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+          if (pass == 1) factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
+#pragma unroll 4
+          for (int c = 0; c < DH / 8; ++c) {
+            const uint4 w = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            uint32_t half2[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float lo = __uint_as_float(u[k] << 16), hi = __uint_as_float(u[k] & 0xFFFF0000u);
+              if (pass == 0)
+                top = fmaxf(top, fmaxf(fabsf(lo), fabsf(hi)));
+              else
+                half2[k] = pack_half(lo * up, hi * up);
+            }
+            if (pass == 1)
+              *reinterpret_cast<uint4*>(smem + L::Q + (c / 8) * L::SUB_BYTES + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = make_uint4(half2[0], half2[1], half2[2], half2[3]);
+          }
+        }
+        factors[row] = factor;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      meet();
+      if (lane == 0) arrive(bar(Q_READY));
+      if (g == 1) factor = factors[row];
+      float m = NOTHING, l = 0.f, ref = 0.f;
+      uint32_t bad[DH / 32] = {};  // dims that a NaN value in this row's sight has
+      bool any_bad = false;
+      // scales: lanes 0 to 7 of a tile's blocks of keys, 8 to 15 of values; pages a tile of this group ahead of that
+      int page = lane < 16 && g < s.n_tiles ? page_of(s, s.key0 / BLOCK + g * TC_BLOCKS + (lane & 7)) : -2;
+      auto scale_of = [&](int i) {
+        if (lane >= 16 || page < 0 || page >= p.n_pages) return lane < 8 ? -1.f : 0.f;
+        const int sub = (s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7)) % page_blocks;
+        return __ldcg(p.scales + ((size_t)(2 * page + (lane >> 3)) * p.n_kv_heads + s.head_kv) * page_blocks + sub);
+      };
+      float scale_ahead = scale_of(g);
+      if (lane < 16) page = g + 2 < s.n_tiles ? page_of(s, s.key0 / BLOCK + (g + 2) * TC_BLOCKS + (lane & 7)) : -2;
+      bool first = true;
+      for (int i = g; i < s.n_tiles && ok; i += 2) {
+        const float scale = scale_ahead;
+        if (i + 2 < s.n_tiles) {
+          scale_ahead = scale_of(i + 2);
+          if (lane < 16) page = i + 4 < s.n_tiles ? page_of(s, s.key0 / BLOCK + (i + 4) * TC_BLOCKS + (lane & 7)) : -2;
+        }
+        const int key0 = s.key0 + i * TC_KEYS;
+        const bool there = __all_sync(0xffffffffu, lane >= 8 || scale >= 0.f);
+        const bool whole = there && is_whole(s, key0);
+        ok = wait(S_FULL + g, s_count & 1u);
+        if (!ok) break;
+        ++s_count;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (some_row) {
+          // the tile's maximum, in units of log 2
+          auto hidden = [&](int key) { return key > qpos || (p.window > 0 && key <= qpos - p.window); };
+          float top = NOTHING, share_top = 0.f;
+          uint32_t ra[16], rb[16];  // two blocks' columns, one on its way while the other is looked at
+          auto look = [&](uint32_t(&x)[16], int b) {
+            const float ks = __shfl_sync(0xffffffffu, scale, b);
+            share_top = fmaxf(share_top, __shfl_sync(0xffffffffu, scale, 8 + b));
+            float y[2] = {NOTHING, NOTHING};
+            if (whole) {
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) y[k / 2 & 1] = max3(y[k / 2 & 1], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+            } else if (ks >= 0.f) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (!hidden(key0 + b * BLOCK + k)) y[0] = fmaxf(y[0], __uint_as_float(x[k]));
+            }
+            const float most = fmaxf(y[0], y[1]);
+            top = most == NOTHING ? top : fmaxf(top, most * (factor * ks));
+          };
+          // (rounds are not unrolled: sixteen warps of three kinds share the instruction cache)
+          tc::tmem_load16(s_at, ra);
+#pragma unroll 1
+          for (int b = 0; b < 8; b += 2) {
+            tmem_wait_load16(ra);
+            tc::tmem_load16(s_at + 16u * (b + 1), rb);
+            look(ra, b);
+            tmem_wait_load16(rb);
+            if (b < 6) tc::tmem_load16(s_at + 16u * (b + 2), ra);
+            look(rb, b + 1);
+          }
+          // the output follows when the maximum has grown by more than 2^8, or a value scale is above the reference
+          const float m_new = top > m + 8.f || m == NOTHING ? fmaxf(m, top) : m;
+          const float ref_new = share_top > ref ? 2.f * share_top : ref;
+          if (__any_sync(0xffffffffu, m_new != m || ref_new != ref)) {
+            const float turn_l = ex2(m - m_new), turn = turn_l * (ref == 0.f ? 0.f : ref * inverse_of(ref_new));
+            l *= turn_l;
+            if (!first) {
+              ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
+              if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for (int c = 0; c < DH; c += 16) {
+                  uint32_t r[16];
+                  tc::tmem_load16(o_at + (uint32_t)(g * DH + c), r);
+                  tmem_wait_load16(r);
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * turn);
+                  tmem_store16(o_at + (uint32_t)(g * DH + c), r);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              }
+            }
+            m = m_new, ref = ref_new;
+          }
+          // Probabilities times share, over the scores that have been read: the share is a power of two and goes into the exponent (2^-60 at
+          // least: what lies below adds nothing to a half), and the sum of a block's is brought back by it.
+          const int ref_e = (int)(__float_as_uint(ref) >> 23);
+          auto weigh = [&](uint32_t(&x)[16], int b) {
+            const float ks = __shfl_sync(0xffffffffu, scale, b), vs = __shfl_sync(0xffffffffu, scale, 8 + b);
+            const int e = max((int)(__float_as_uint(vs) >> 23) - ref_e + 7, -60);
+            const float f = factor * ks, from = (float)e - m, back = __uint_as_float((uint32_t)(127 - e) << 23);
+            uint32_t packed[8];
+            if (whole) {
+              const uint64_t f2 = pair(f, f), from2 = pair(from, from);
+              uint64_t sum2 = 0ull;
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const uint64_t y = fma2((uint64_t)x[k] | ((uint64_t)x[k + 1] << 32), f2, from2);
+                const float x0 = ex2(__uint_as_float((uint32_t)y)), x1 = ex2(__uint_as_float((uint32_t)(y >> 32)));
+                sum2 = add2(sum2, pair(x0, x1));
+                packed[k / 2] = pack_half(x0, x1);
+              }
+              l = fmaf(__uint_as_float((uint32_t)sum2) + __uint_as_float((uint32_t)(sum2 >> 32)), back, l);
+            } else {
+              float sum = 0.f;
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const int key = key0 + b * BLOCK + k;
+                const float x0 = ks < 0.f || hidden(key) ? 0.f : ex2(fmaf(__uint_as_float(x[k]), f, from));
+                const float x1 = ks < 0.f || hidden(key + 1) ? 0.f : ex2(fmaf(__uint_as_float(x[k + 1]), f, from));
+                sum += x0 + x1;
+                packed[k / 2] = pack_half(x0, x1);
+              }
+              l = fmaf(sum, back, l);
+            }
+            tmem_store8(s_at + 8u * b, packed);
+          };
+          tc::tmem_load16(s_at, ra);
+#pragma unroll 1
+          for (int b = 0; b < 8; b += 2) {
+            tmem_wait_load16(ra);
+            tc::tmem_load16(s_at + 16u * (b + 1), rb);
+            weigh(ra, b);
+            tmem_wait_load16(rb);
+            if (b < 6) tc::tmem_load16(s_at + 16u * (b + 2), ra);
+            weigh(rb, b + 1);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        if (!whole && ok) {  // values that are NaN, of the keys that this row sees
+          const uint32_t stage = (v_count + (uint32_t)i) & 1u;
+          ok = wait(V_FULL + (int)stage, ((v_count + (uint32_t)i) >> 1) & 1u);
+          int some = 0;
+          {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) some |= reinterpret_cast<const int*>(smem + L::NAN_SOME)[stage * 4 + k];
+          }
+          if (ok && some) {
+            const uint32_t* bits = reinterpret_cast<const uint32_t*>(smem + L::NAN_BITS) + stage * (TC_KEYS * (DH / 32));
+            for (int k = 0; k < TC_KEYS; ++k) {
+              const bool hidden = __shfl_sync(0xffffffffu, scale, k / BLOCK) < 0.f || key0 + k > qpos || (p.window > 0 && key0 + k <= qpos - p.window);
+#pragma unroll
+              for (int d = 0; d < DH / 32; ++d) bad[d] |= hidden ? 0u : bits[k * (DH / 32) + d];
+            }
+            any_bad = true;
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && ok) arrive(bar(P_READY + g));
+        ++pv_count;
+        first = false;
+      }
+      v_count += (uint32_t)s.n_tiles;
+      // the unit's end: both groups' outputs, each group half of the columns
+      if (ok && !first) ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
+      ml[g * 128 + row] = make_float4(m, l, ref, first ? 0.f : 1.f);
+      uint32_t* bad_at = reinterpret_cast<uint32_t*>(smem + L::Q) + row * (DH / 32);  // [group][row]: the queries are used
+      const bool bad_somewhere = !all_of_us(!any_bad);
+      if (bad_somewhere) {
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) bad_at[g * 128 * (DH / 32) + d] = bad[d];
+        meet();
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (ok && some_row) {
+        const float4 a = ml[row], b = ml[128 + row];
+        const float top = fmaxf(a.x, b.x), fa = ex2(a.x - top), fb = ex2(b.x - top), sum = a.y * fa + b.y * fb;
+        const float scale = s.part < 0 ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+        const float ua = fa * scale * (a.z * 0.0078125f), ub = fb * scale * (b.z * 0.0078125f);  // ref * 2^-7
+        const size_t part_row = (size_t)s.part * TC_ROWS + row;
+        const size_t to = s.part < 0 ? (size_t)(s.token0 + q) * p.out_stride + (size_t)h * DH : part_row * DH;
+#pragma unroll 1
+        for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
+          uint32_t ra[16], rb[16];
+          tc::tmem_load16(o_at + (uint32_t)c, ra);
+          tc::tmem_load16(o_at + (uint32_t)(DH + c), rb);
+          tmem_wait_load16(ra);
+          tmem_wait_load16(rb);
+          float o[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = (a.w != 0.f ? __uint_as_float(ra[k]) * ua : 0.f) + (b.w != 0.f ? __uint_as_float(rb[k]) * ub : 0.f);
+          if (bad_somewhere) {
+            const uint32_t word = (bad_at[c / 32] | bad_at[128 * (DH / 32) + c / 32]) >> (c % 32);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if ((word >> k) & 1u) o[k] = CUDART_NAN_F;
+          }
+          if (row_ok) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              if (s.part < 0)
+                store4<false>(p.out, to + c + k, o[k], o[k + 1], o[k + 2], o[k + 3]);
+              else
+                *reinterpret_cast<float4*>(p.part_o + to + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            }
+          }
+        }
+        if (s.part >= 0 && row_ok && g == 0) *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(top, sum);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(bar(O_FREE));
+      done_with(n);
+    }
+  } else if (warp == 12) {
+    // ---- products: the whole warp walks, one lane issues ----
+    constexpr uint32_t idesc_s = tc_instr_desc(TC_KEYS, false), idesc_o = tc_instr_desc(DH, true);
+    const uint64_t q_desc = tc::smem_desc(base + L::Q), k_desc = tc::smem_desc(base + L::K), v_desc = tc_desc_mn(base + L::V);
+    uint32_t count = 0, p_count[2] = {0, 0};
+    TcSegment s;
+    bool ok = true;
+    for (uint32_t n = 0; ok && next_segment(n, s); ++n) {
+      ok = wait(Q_READY, n & 1u);
+      auto issue_s = [&](int i) {  // scores of tile i, over the probabilities that the group's tile before has left there
+        const int g = i & 1;
+        const uint32_t stage = (count + (uint32_t)i) & 1u;
+        if (p_count[g] > 0) ok = wait(PV_DONE + g, (p_count[g] - 1u) & 1u);
+        if (ok) ok = wait(K_FULL + (int)stage, ((count + (uint32_t)i) >> 1) & 1u);
+        if (!ok) return;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int k = 0; k < DH / 16; ++k) {  // descriptors count 16-byte units: a step of 16 halves is 2
+            const uint64_t off = (uint64_t)((k / 4) * (L::SUB_BYTES >> 4) + (k % 4) * 2);
+            tc::mma_f16(tmem + (uint32_t)g * 128u, q_desc + off, k_desc + (uint64_t)(stage * (L::MAT >> 4)) + off, idesc_s, k != 0 ? 1u : 0u);
+          }
+          tc::mma_commit(bar(K_EMPTY + (int)stage));
+          tc::mma_commit(bar(S_FULL + g));
+        }
+        __syncwarp();
+      };
+      if (ok) issue_s(0);
+      if (ok && s.n_tiles > 1) issue_s(1);
+      for (int i = 0; i < s.n_tiles && ok; ++i) {
+        const int g = i & 1;
+        const uint32_t stage = (count + (uint32_t)i) & 1u;
+        if (i == 0 && n > 0) ok = wait(O_FREE, (n - 1u) & 1u);
+        if (ok) ok = wait(P_READY + g, p_count[g] & 1u);
+        if (ok) ok = wait(V_FULL + (int)stage, ((count + (uint32_t)i) >> 1) & 1u);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int k = 0; k < TC_KEYS / 16; ++k)  // 16 keys: eight columns of packed probabilities, 16 rows of values
+            mma_from_tmem(tmem + 256u + (uint32_t)(g * DH), tmem + (uint32_t)(g * 128 + k * 8), v_desc + (uint64_t)(stage * (L::MAT >> 4) + k * (2048 >> 4)), idesc_o,
+                          i >= 2 || k != 0 ? 1u : 0u);
+          tc::mma_commit(bar(V_EMPTY + (int)stage));
+          tc::mma_commit(bar(PV_DONE + g));
+        }
+        __syncwarp();
+        ++p_count[g];
+        if (i + 2 < s.n_tiles) issue_s(i + 2);
+      }
+      count += (uint32_t)s.n_tiles;
+      done_with(n);
+    }
+  } else {
+    // ---- which tiles come next ----
+    uint32_t told = 0;
+    bool ok = true;
+    auto say = [&](const TcSegment& s) {
+      const uint32_t turn = told & 1u;
+      if (told >= 2) ok = wait(SEG_EMPTY + (int)turn, ((told >> 1) & 1u) ^ 1u);
+      if (ok && lane == 0) {
+        segments[turn] = s;
+        arrive(bar(SEG_FULL + (int)turn));
+      }
+      __syncwarp();
+      ++told;
+    };
+    for (; at < end && ok; ++entry) {
+      const Work w = work_of<TC_ROWS>(p, entry);
+      const int tiles = w.tiles(TC_BLOCKS);
+      if (tiles == 0) continue;
+      int h = rest / (p.cost + tiles), off = rest - h * (p.cost + tiles);
+      rest = 0;
+      for (; h < p.n_kv_heads && at < end && ok; ++h) {
+        const int n = min(p.cost + tiles - off, end - at), i0 = max(off - p.cost, 0), i1 = max(off + n - p.cost, 0);
+        if (i1 > i0)
+          say(TcSegment{i1 - i0, (w.first_block + i0 * TC_BLOCKS) * BLOCK, i1 - i0 == tiles ? -1 : (int)blockIdx.x * 2 + (off >= p.cost ? 0 : 1), w.token0,
+                        w.pos0, w.first_row, w.rows, h, w.slot, w.first_seen, w.first_block + w.n_blocks, w.pos0 + w.first_row / group,
+                        w.pos0 + (w.first_row + w.rows - 1) / group, {}});
+        at += n;
+        off = 0;
+      }
+    }
+    if (ok) say(TcSegment{-1});
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+template <int DH>
+int launch_attention_tc(AttnParams8 p, int blocks, cudaStream_t stream) {
+  using L = TcLayout<DH>;
+  static_assert(L::BYTES <= 227 * 1024, "shared memory");
+  if ((p.n_entries + 1) * 4 > 2 * L::MAT) return -10;  // the keys' place holds the entries' tiles at first
+  const auto kernel = kv8_attention_tc_kernel<DH>;
+  const int rc = (int)note_launch(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
+  if (rc != 0) return take_launch_error();
+  p.cost = 2;
+  launch_pdl_split(false, kernel, dim3(blocks), dim3(TC_THREADS), L::BYTES, stream, p);
+  launch_pdl(kv8_join_kernel<false, TC_ROWS>, dim3(p.n_entries, p.n_kv_heads), dim3(128), 0, stream, p);
+  return 0;
+}
+
+}  // namespace kv8
+}  // namespace rl

@@ -2151,9 +2151,18 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
         return have
     rows = queries * (n_heads // n_kv)
     block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
+    if kv8_on_tcgen05(code, rows, dh):
+        block = 128
     row_blocks = -(-rows // block)
     entries = n_items * row_blocks
     sms = sm_count()
+    if block == 128 and entries <= KV8_MOST_ENTRIES:
+        plan = -(-(entries + 2) // 4) * 4
+        have = _KV8_PLANS[key] = (block, row_blocks, sms, sms, plan, plan + sms * 2 * block * (dh + 2))
+        return have
+    if block == 128:
+        block, row_blocks = 64, -(-rows // 64)
+        entries = n_items * row_blocks
     at_once = sms * _lib().rl_kv8_attention_blocks(code, block, is_tiles, n_heads, n_kv, dh)
     if _kv8_by_units(dh, span) or entries > KV8_MOST_ENTRIES:
         have = (block, row_blocks, 0, 0, 0, 0)
@@ -2166,6 +2175,11 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
     return have
 
 
+def kv8_on_tcgen05(code: int, rows: int, dh: int) -> bool:
+    return code == BF16 and dh in (64, 128) and rows > KV8_TC_ROWS
+
+
+KV8_TC_ROWS = 16
 KV8_MOST_ENTRIES = 4096  # blocks of rows whose keys are shared evenly: their numbers lie in shared memory once
 
 
