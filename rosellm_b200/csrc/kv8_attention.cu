@@ -24,7 +24,7 @@ RL_EXPORT int rl_kv8_attention_blocks(int dtype, int rows, int is_tiles, int n_h
 }
 
 // items: decoded requests int32 [n_items], or (is_tiles) int32 [n_items][2] = (request, first query) of 64-query tiles.  rows: of a block of
-// threads, 8, 16, 32 or 64, or 128 (tcgen05: bfloat16, head sizes 64 and 128, sms not 0); row_blocks: of an item and key/value head.  sms 0: a block of threads to every unit; else `blocks` of them share all units' tiles
+// threads, 8, 16, 32 or 64, or 128 (tcgen05: bfloat16, head sizes 64 and 128, pages of up to 4096 tokens, sms not 0); row_blocks: of an item and key/value head.  sms 0: a block of threads to every unit; else `blocks` of them share all units' tiles
 // evenly (sms of them where there is little to do), plan holds n_items * row_blocks + 2 ints, part_o blocks * 2 * rows * head_dim floats and part_ml
 // two for every head_dim of those.
 RL_EXPORT int rl_kv8_attention(int dtype, const void* q, long q_stride, const void* pool, const float* scales, const int* block_table,
@@ -37,7 +37,7 @@ RL_EXPORT int rl_kv8_attention(int dtype, const void* q, long q_stride, const vo
   if (n_kv_heads <= 0 || n_heads % n_kv_heads != 0) return -3;
   if (page_size <= 0 || page_size % rl::kv8::BLOCK != 0) return -4;
   if (row_blocks < 1 || sms < 0 || (rows != 8 && rows != 16 && rows != 32 && rows != 64 && rows != 128)) return -5;
-  if (rows == 128 && (dtype != RL_BF16 || sms <= 0 || (head_dim != 64 && head_dim != 128))) return -5;
+  if (rows == 128 && (dtype != RL_BF16 || sms <= 0 || (head_dim != 64 && head_dim != 128) || page_size > 4096)) return -5;
   if (n_kv_heads > 65535 || (long)n_items * row_blocks > 0x7fffffffL) return -6;
   if (sms > 0 && (blocks < 1 || plan == nullptr || part_o == nullptr || part_ml == nullptr)) return -7;
   if (status == nullptr) return -8;

@@ -74,7 +74,9 @@ __device__ __forceinline__ Work work_of(const AttnParams8& p, int entry) {
   w.req = p.is_tiles ? p.items[2 * item] : p.items[item];
   const int t0 = p.is_tiles ? p.items[2 * item + 1] : 0;
   const int qs = p.q_start[w.req], q_len = p.q_start[w.req + 1] - qs, kv_len = p.kv_len[w.req];
-  const int n_q = min(p.is_tiles ? TILE_QUERIES : 1, q_len - t0);
+  // (blocks of 128 rows of heads that stand alone take two tiles of 64 queries at once: the first of them both, the second nothing)
+  const bool doubled = RB == 2 * TILE_QUERIES && group == 1 && p.is_tiles;
+  const int n_q = doubled && t0 % (2 * TILE_QUERIES) != 0 ? 0 : min(!p.is_tiles ? 1 : doubled ? 2 * TILE_QUERIES : TILE_QUERIES, q_len - t0);
   w.first_row = (entry - item * p.row_blocks) * RB;
   w.rows = min(RB, n_q * group - w.first_row);
   w.token0 = qs + t0;
@@ -908,7 +910,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
 }
 
 // Joins the parts of the units that lie in several runs, in the order of the keys: m = max m_k, o = sum o_k 2^(m_k - m) / sum l_k 2^(m_k - m).
-// grid: entries, key/value heads.
+// grid: entries, key/value heads, eights of rows.
 template <bool F32, int RB>
 __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   pdl_begin();
@@ -920,9 +922,9 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   const Rows rows{w.token0, w.pos0, w.first_row, w.rows, (int)blockIdx.y};
   // a block's part lies in the first of its two places if its run begins among the unit's tiles, else in the second
   auto part_row = [&](int k, int row) { return ((size_t)(first + k) * 2 + ((long)(first + k) * run < begin ? 1 : 0)) * RB + row; };
-  const int quads = p.head_dim / 4;
-  for (int i = threadIdx.x; i < w.rows * quads; i += 128) {
-    const int row = i / quads, d = i % quads * 4;
+  const int quads = p.head_dim / 4, row0 = blockIdx.z * 8, n_rows = min(8, w.rows - row0);
+  for (int i = threadIdx.x; i < n_rows * quads; i += 128) {
+    const int row = row0 + i / quads, d = i % quads * 4;
     float m = NOTHING, l = 0.f;
     for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[part_row(k, row) * 2]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -983,7 +985,7 @@ int launch_attention(AttnParams8 p, int most_rows, int blocks, Fit* fit, cudaStr
   const int rc = (int)note_launch(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f.bytes));
   if (rc != 0) return take_launch_error();
   launch_pdl_all_shared(kernel, p.balanced ? dim3(blocks) : dim3(p.n_entries, p.n_kv_heads), dim3(160), f.bytes, stream, p);
-  if (p.balanced) launch_pdl(kv8_join_kernel<F32, L::RB>, dim3(p.n_entries, p.n_kv_heads), dim3(128), 0, stream, p);
+  if (p.balanced) launch_pdl(kv8_join_kernel<F32, L::RB>, dim3(p.n_entries, p.n_kv_heads, L::RB / 8), dim3(128), 0, stream, p);
   return 0;
 }
 

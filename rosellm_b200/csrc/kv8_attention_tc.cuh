@@ -1,12 +1,12 @@
 // Attention over the 8-bit cache on tcgen05, for many rows (bfloat16, head sizes 64 and 128): the function of kv8_attention.cuh.
 //
 // A block of threads takes 128 rows, queries times the heads that share one key/value head, and walks their keys in tiles of 128.  Its warps:
-//   0-3    bring codes from memory to registers, a tile ahead, turn them into halves (exact) and write those into the swizzled layouts that the
+//   0-7    bring codes from memory to registers, a tile ahead, turn them into halves (exact) and write those into the swizzled layouts that the
 //          products read, keys and values apart, two stages of each;
-//   4-11   softmax, two groups of four warps on alternate tiles, a thread a row: read the scores from tensor memory, write the
-//          probabilities back over them as halves.  Each group has a maximum, a sum and an output of its own; they meet at the end of the unit;
-//   12     issues S = Q K^T (M 128, N 128) and O += P V (P taken from tensor memory, V as it lies);
-//   13     says which tiles of which unit come next.
+//   8-15   softmax, two groups of four warps on alternate tiles, a thread a row: read the scores from tensor memory, write the
+//          probabilities back over them as halves (head 64: beside them).  Each group has a maximum, a sum and an output of its own; they meet at the end of the unit;
+//   16     issues S = Q K^T (M 128, N 128) and O += P V (P taken from tensor memory, V as it lies);
+//   17     says which tiles of which unit come next.
 // Tensor memory: two tiles of scores, 128 columns each, and two outputs of head dim columns.
 //
 // Scales as in kv8_attention.cuh: a block of 16 keys is 16 columns of the scores, so a key scale is a factor of 16 columns' exponents and a value
@@ -22,24 +22,27 @@
 namespace rl {
 namespace kv8 {
 
-constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_BLOCKS = TC_KEYS / BLOCK, TC_THREADS = 448;
+constexpr int TC_ROWS = 128, TC_KEYS = 128, TC_BLOCKS = TC_KEYS / BLOCK, TC_THREADS = 576;
 
 template <int DH>
 struct TcLayout {
   static constexpr int SUBS = DH / 64;                 // stretches of 64 entries, 128 bytes of halves: a row of the swizzle
   static constexpr int SUB_BYTES = 128 * 128;          // 128 rows of one
+  // tensor memory: scores at 0 and 128, outputs at 256 and 256 + DH, probabilities (64 columns) over the group's scores, or behind all where there is room
+  static constexpr bool P_APART = DH == 64;
+  __device__ __forceinline__ static uint32_t p_col(int g) { return P_APART ? 384u + 64u * (uint32_t)g : 128u * (uint32_t)g; }
   static constexpr int MAT = SUBS * SUB_BYTES;
   static constexpr int Q = 0, K = MAT, V = K + 2 * MAT;
   static constexpr int NAN_BITS = V + 2 * MAT;         // [stage][key][DH / 16] a bit for each value of a tile that not every row sees whole: NaN
-  static constexpr int NAN_SOME = NAN_BITS + 2 * TC_KEYS * (DH / 8);  // [stage][4 warps]: whether there is one
-  static constexpr int ML = NAN_SOME + 2 * 4 * 4;      // [group][128 rows] maximum, sum, reference, whether there is anything
+  static constexpr int NAN_SOME = NAN_BITS + 2 * TC_KEYS * (DH / 8);  // [stage][8 warps]: whether there is one
+  static constexpr int ML = NAN_SOME + 2 * 8 * 4;      // [group][128 rows] maximum, sum, reference, whether there is anything
   static constexpr int FACTOR = ML + 2 * 128 * 16;     // [128 rows]
   static constexpr int SEG = FACTOR + 512;             // two segments
   static constexpr int BARS = SEG + 2 * 64;
   static constexpr int BYTES = BARS + 8 * 24 + 16 + 1024;  // and room to align
 };
 
-enum TcBar { SEG_FULL = 0, SEG_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY = 10, S_FULL = 12, P_READY = 14, PV_DONE = 16, Q_READY = 18, O_FREE = 19, TC_BARS = 20 };
+enum TcBar { SEG_FULL = 0, SEG_EMPTY = 2, K_FULL = 4, K_EMPTY = 6, V_FULL = 8, V_EMPTY = 10, S_FULL = 12, P_READY = 14, PV_DONE = 16, Q_READY = 18, O_FREE = 19, WEIGHED = 20, TC_BARS = 22 };
 
 __device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -66,6 +69,14 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
 __device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
                "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
                : "memory");
 }
 __device__ __forceinline__ void tmem_wait_load16(uint32_t (&r)[16]) {
@@ -105,6 +116,8 @@ struct TcSegment {
   int pad[3];
 };
 
+// Registers: 576 threads are launched with 96 each; eight warps that convert give 24 each to eight that do the softmax (8 * 72 + 8 * 120 + 2 * 96 =
+// 18 * 96, two of each on every quarter of the SM).
 template <int DH>
 __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const AttnParams8 p) {
   using L = TcLayout<DH>;
@@ -119,14 +132,15 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(bar(SEG_FULL + i), 1);
-      tc::mbar_init(bar(SEG_EMPTY + i), 13);
-      tc::mbar_init(bar(K_FULL + i), 4);
+      tc::mbar_init(bar(SEG_EMPTY + i), 17);
+      tc::mbar_init(bar(K_FULL + i), 8);
       tc::mbar_init(bar(K_EMPTY + i), 1);
-      tc::mbar_init(bar(V_FULL + i), 4);
+      tc::mbar_init(bar(V_FULL + i), 8);
       tc::mbar_init(bar(V_EMPTY + i), 1);
       tc::mbar_init(bar(S_FULL + i), 1);
       tc::mbar_init(bar(P_READY + i), 4);
       tc::mbar_init(bar(PV_DONE + i), 1);
+      tc::mbar_init(bar(WEIGHED + i), 4);
     }
     tc::mbar_init(bar(Q_READY), 8);
     tc::mbar_init(bar(O_FREE), 8);
@@ -134,7 +148,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -146,7 +160,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     before[e] = tiles > 0 ? p.cost + tiles : 0;
   }
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     int sum = 0;
     for (int e = 0; e < p.n_entries; e += 32) {
       int x = e + lane < p.n_entries ? before[e + lane] : 0;
@@ -165,7 +179,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   }
   // the run of this block, before the numbers' place is written over
   int at = 0, end = 0, entry = 0, rest = 0;
-  if (warp == 13) {
+  if (warp == 17) {
     const int total = before[p.n_entries] * p.n_kv_heads, blocks = (int)gridDim.x;
     const int run = max((total + blocks - 1) / blocks, p.cost + 1);
     if (blockIdx.x == 0) {  // for the kernel that joins
@@ -188,6 +202,9 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int group = p.n_heads / p.n_kv_heads, page_blocks = p.page_size / BLOCK;
+  // b / page_blocks for block numbers below 2^24 and pages of up to 256 blocks: the high half of b * (2^32 / page_blocks + 1)
+  const uint32_t per_page = page_blocks > 1 ? 0xFFFFFFFFu / (uint32_t)page_blocks + 1u : 0u;
+  auto page_index = [&](int b) { return per_page != 0u ? (int)__umulhi((uint32_t)b, per_page) : b; };
   auto wait = [&](int which, uint32_t parity) { return tc::mbar_wait_warp(bar(which), parity, abort_flag, p.status); };
   // The segment at hand, for the roles below; false when there is none.
   auto next_segment = [&](uint32_t n, TcSegment& s) {
@@ -203,7 +220,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   };
   auto page_of = [&](const TcSegment& s, int b) {  // of block b; -1: none, -2: not wanted
     if (b < s.first_seen || b >= s.end_block) return -2;
-    const int e = b / page_blocks;
+    const int e = page_index(b);
     return s.slot >= 0 && s.slot < p.bt_rows && e < p.bt_cols ? p.block_table[(size_t)s.slot * p.bt_cols + e] : -1;
   };
   // whether every row of the block of threads sees every key of a tile
@@ -211,13 +228,16 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     return key0 + TC_KEYS - 1 <= s.pos_lo && (p.window <= 0 || key0 > s.pos_hi - p.window) && key0 >= s.first_seen * BLOCK;
   };
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---- codes to halves ----
-    constexpr int PIECES = DH / 16;                    // of 16 codes, a thread, of the keys of a tile
-    constexpr int APART = 128 / DH;                    // blocks of 16 keys between two of a thread's pieces
-    const int t = threadIdx.x, own_block = t / DH, key_in_block = t % DH / (DH / 16), part = t % (DH / 16);
-    const size_t to_values = (size_t)p.n_kv_heads * p.page_size * DH;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+    constexpr int PIECES = DH / 32;                    // of 16 codes, a thread, of the keys of a tile
+    constexpr int APART = 256 / DH;                    // blocks of 16 keys between two of a thread's pieces
+    // four neighbouring lanes take 64 codes of a key, the next four the same of the next key: eight lanes then write all of the banks
+    const int t = threadIdx.x, key_in_block = t / 4 % 16, part = t % 4 + (DH == 128 ? t / 64 % 2 * 4 : 0), own_block = t / DH;
+    const int to_values = p.n_kv_heads * page_blocks;  // blocks of 16 keys from a block of keys to that of its values
     const int in_block = key_in_block * DH + part * 16;
+    const uint8_t* own_pool = p.pool + in_block;
     // where the piece's halves go: a row of 128 bytes a key, 16-byte pieces swizzled by the key (key % 8 is that of key_in_block)
     const uint32_t own_row = (uint32_t)(part / 4) * L::SUB_BYTES + (uint32_t)(own_block * BLOCK + key_in_block) * 128u;
     const uint32_t own_chunk = (uint32_t)((part % 4 * 2) ^ (key_in_block & 7)) << 4;
@@ -226,23 +246,21 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     TcSegment s;
     bool ok = true;
     for (uint32_t n = 0; ok && next_segment(n, s); ++n) {
-      // lanes look after a tile's eight blocks (lane % 8): the table's entry, and from it where the block's keys lie (of a block that is not there,
-      // the pool's first: what is read is hidden from every row, and its values are looked through for NaN)
+      // lanes look after a tile's eight blocks (lane % 8): the table's entry, and from it which of the pool's blocks has its keys (of a block that
+      // is not there, the first: what is read is hidden from every row, and its values are looked through for NaN)
       auto look_up = [&](int i) { return i < s.n_tiles ? page_of(s, s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7)) : -2; };
-      auto place_of = [&](int page, int i) -> const uint8_t* {
+      auto place_of = [&](int page, int i) {
         if (page != -2 && (page < 0 || page >= p.n_pages)) {
           atomicOr(p.status, RL_STATUS_BAD_PAGE);
           page = -1;
         }
         const int b = s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7);
-        return page < 0 ? p.pool : p.pool + (((size_t)page * 2 * p.n_kv_heads + s.head_kv) * p.page_size + b % page_blocks * BLOCK) * DH;
+        return page < 0 ? 0 : (page * 2 * p.n_kv_heads + s.head_kv) * page_blocks + b - page_index(b) * page_blocks;
       };
-      auto load = [&](uint4(&to)[PIECES], const uint8_t* place, size_t plane) {
+      auto load = [&](uint4(&to)[PIECES], int place, int plane) {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-          const uint8_t* from = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), own_block + APART * j));
-          to[j] = __ldcg(reinterpret_cast<const uint4*>(from + plane + in_block));
-        }
+        for (int j = 0; j < PIECES; ++j)
+          to[j] = __ldcg(reinterpret_cast<const uint4*>(own_pool + (size_t)(uint32_t)(__shfl_sync(0xffffffffu, place, own_block + APART * j) + plane) * (BLOCK * DH)));
       };
       // 16 codes as two 16-byte pieces of a row of halves
       auto store = [&](uint32_t mat, int j, const uint4& codes) {
@@ -289,7 +307,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
             some |= found;
           }
           const bool any = __any_sync(0xffffffffu, some != 0u);
-          if (lane == 0) reinterpret_cast<int*>(smem + L::NAN_SOME)[stage * 4 + warp] = any;
+          if (lane == 0) reinterpret_cast<int*>(smem + L::NAN_SOME)[stage * 8 + warp] = any;
         }
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) store(base + L::V + stage * L::MAT, j, from[j]);
@@ -301,7 +319,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       const int e0 = look_up(0), e1 = look_up(1), e2 = look_up(2);
       int entry_ahead = look_up(3);
       // places of the values of the next tiles: keys are three tiles ahead when they are loaded
-      const uint8_t *v0 = place_of(e0, 0), *v1 = place_of(e1, 1), *v2 = place_of(e2, 2);
+      int v0 = place_of(e0, 0), v1 = place_of(e1, 1), v2 = place_of(e2, 2);
       bool t0 = all_there(e0), t1 = all_there(e1), t2 = all_there(e2);
       load(keys, v0, 0);
       load(values, v0, to_values);
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         convert_values(values, i, t0);
         load(values, v1, to_values);
         if (i + 2 < s.n_tiles) convert_keys(keys, i + 2);
-        const uint8_t* v3 = place_of(entry_ahead, i + 3);
+        const int v3 = place_of(entry_ahead, i + 3);
         load(keys, v3, 0);
         v1 = v2, v2 = v3;
         t0 = t1, t1 = t2, t2 = all_there(entry_ahead);
@@ -323,11 +341,12 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       count += (uint32_t)s.n_tiles;
       done_with(n);
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ---- softmax ----
-    const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;" ::: "memory");
+    const int g = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_at = tmem + lanes + (uint32_t)g * 128u, o_at = tmem + lanes + 256u;
+    const uint32_t s_at = tmem + lanes + (uint32_t)g * 128u, o_at = tmem + lanes + 256u, p_at = tmem + lanes + L::p_col(g);
     auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
     auto all_of_us = [&](bool mine) {
       uint32_t all;
@@ -336,7 +355,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     };
     float4* ml = reinterpret_cast<float4*>(smem + L::ML);
     float* factors = reinterpret_cast<float*>(smem + L::FACTOR);
-    uint32_t s_count = 0, pv_count = 0, v_count = 0;  // of this group's tiles; of all tiles (stages go by them)
+    uint32_t s_count = 0, pv_count = 0, v_count = 0, others = 0;  // of this group's tiles; of all tiles (stages go by them); of the other group's
     TcSegment s;
     bool ok = true;
     for (uint32_t n = 0;; ++n) {
@@ -348,28 +367,26 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       float factor = 0.f;
       if (g == 0) {  // this row's queries as halves, by a power of two that puts the largest entry between 2^14 and 2^15
         const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)(s.token0 + q) * p.q_stride + (size_t)h * DH);
-        float top = 0.f;
-#pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 126);
-          const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-          if (pass == 1) factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
-#pragma unroll 4
-          for (int c = 0; c < DH / 8; ++c) {
-            const uint4 w = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-            uint32_t half2[4];
+        uint4 w[DH / 8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float lo = __uint_as_float(u[k] << 16), hi = __uint_as_float(u[k] & 0xFFFF0000u);
-              if (pass == 0)
-                top = fmaxf(top, fmaxf(fabsf(lo), fabsf(hi)));
-              else
-                half2[k] = pack_half(lo * up, hi * up);
-            }
-            if (pass == 1)
-              *reinterpret_cast<uint4*>(smem + L::Q + (c / 8) * L::SUB_BYTES + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = make_uint4(half2[0], half2[1], half2[2], half2[3]);
-          }
+        for (int c = 0; c < DH / 8; ++c) w[c] = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < DH / 8; ++c) {
+          const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max3(top, fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xFFFF0000u)));
+        }
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 126);
+        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+        factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int c = 0; c < DH / 8; ++c) {
+          const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+          uint32_t half2[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) half2[k] = pack_half(__uint_as_float(u[k] << 16) * up, __uint_as_float(u[k] & 0xFFFF0000u) * up);
+          *reinterpret_cast<uint4*>(smem + L::Q + (c / 8) * L::SUB_BYTES + row * 128 + (((c % 8) ^ (row & 7)) << 4)) = make_uint4(half2[0], half2[1], half2[2], half2[3]);
         }
         factors[row] = factor;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       int page = lane < 16 && g < s.n_tiles ? page_of(s, s.key0 / BLOCK + g * TC_BLOCKS + (lane & 7)) : -2;
       auto scale_of = [&](int i) {
         if (lane >= 16 || page < 0 || page >= p.n_pages) return lane < 8 ? -1.f : 0.f;
-        const int sub = (s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7)) % page_blocks;
+        const int b = s.key0 / BLOCK + i * TC_BLOCKS + (lane & 7), sub = b - page_index(b) * page_blocks;
         return __ldcg(p.scales + ((size_t)(2 * page + (lane >> 3)) * p.n_kv_heads + s.head_kv) * page_blocks + sub);
       };
       float scale_ahead = scale_of(g);
@@ -399,40 +416,64 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         const int key0 = s.key0 + i * TC_KEYS;
         const bool there = __all_sync(0xffffffffu, lane >= 8 || scale >= 0.f);
         const bool whole = there && is_whole(s, key0);
+        // of the eight blocks: what scores are multiplied by, and the value scales' exponents
+        float f[8], share_top = 0.f;
+        int ve[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const float ks = __shfl_sync(0xffffffffu, scale, b), vs = __shfl_sync(0xffffffffu, scale, 8 + b);
+          f[b] = factor * ks;
+          ve[b] = (int)(__float_as_uint(vs) >> 23) + 7;
+          share_top = fmaxf(share_top, vs);
+        }
         ok = wait(S_FULL + g, s_count & 1u);
         if (!ok) break;
         ++s_count;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (some_row) {
           // the tile's maximum, in units of log 2
-          auto hidden = [&](int key) { return key > qpos || (p.window > 0 && key <= qpos - p.window); };
-          float top = NOTHING, share_top = 0.f;
-          uint32_t ra[16], rb[16];  // two blocks' columns, one on its way while the other is looked at
-          auto look = [&](uint32_t(&x)[16], int b) {
-            const float ks = __shfl_sync(0xffffffffu, scale, b);
-            share_top = fmaxf(share_top, __shfl_sync(0xffffffffu, scale, 8 + b));
-            float y[2] = {NOTHING, NOTHING};
-            if (whole) {
+          // (columns from lo_vis to hi_vis - 1 are of keys that the row sees)
+          const int hi_vis = qpos - key0 + 1, lo_vis = p.window > 0 ? qpos - p.window + 1 - key0 : 0;
+          float top = NOTHING;
+          uint32_t ra[32], rb[32];  // two blocks' columns each, one on its way while the other is used
+          auto most_of = [&](const uint32_t(&x)[32], int b) {
 #pragma unroll
-              for (int k = 0; k < 16; k += 2) y[k / 2 & 1] = max3(y[k / 2 & 1], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-            } else if (ks >= 0.f) {
+            for (int h = 0; h < 2; ++h) {
+              float y[2] = {NOTHING, NOTHING};
 #pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (!hidden(key0 + b * BLOCK + k)) y[0] = fmaxf(y[0], __uint_as_float(x[k]));
+              for (int k = 0; k < 16; k += 2) y[k / 2 & 1] = max3(y[k / 2 & 1], __uint_as_float(x[16 * h + k]), __uint_as_float(x[16 * h + k + 1]));
+              top = fmaxf(top, fmaxf(y[0], y[1]) * f[b + h]);
             }
-            const float most = fmaxf(y[0], y[1]);
-            top = most == NOTHING ? top : fmaxf(top, most * (factor * ks));
           };
-          // (rounds are not unrolled: sixteen warps of three kinds share the instruction cache)
-          tc::tmem_load16(s_at, ra);
+          if (whole) {
+            tc::tmem_load32(s_at, ra);
+            tmem_wait_load(ra);
+            tc::tmem_load32(s_at + 32u, rb);
+            most_of(ra, 0);
+            tmem_wait_load(rb);
+            tc::tmem_load32(s_at + 64u, ra);
+            most_of(rb, 2);
+            tmem_wait_load(ra);
+            tc::tmem_load32(s_at + 96u, rb);
+            most_of(ra, 4);
+            tmem_wait_load(rb);
+            most_of(rb, 6);
+          } else {
 #pragma unroll 1
-          for (int b = 0; b < 8; b += 2) {
-            tmem_wait_load16(ra);
-            tc::tmem_load16(s_at + 16u * (b + 1), rb);
-            look(ra, b);
-            tmem_wait_load16(rb);
-            if (b < 6) tc::tmem_load16(s_at + 16u * (b + 2), ra);
-            look(rb, b + 1);
+            for (int b = 0; b < 8; b += 2) {
+              const float k0 = __shfl_sync(0xffffffffu, scale, b), k1 = __shfl_sync(0xffffffffu, scale, b + 1);
+              tc::tmem_load32(s_at + 16u * b, ra);
+              tmem_wait_load(ra);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float ks = h ? k1 : k0;
+                const int lo = lo_vis - (b + h) * BLOCK, hi = ks < 0.f ? 0 : hi_vis - (b + h) * BLOCK;
+                float y = NOTHING;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) y = k >= lo && k < hi ? fmaxf(y, __uint_as_float(ra[16 * h + k])) : y;
+                top = y == NOTHING ? top : fmaxf(top, y * (factor * ks));
+              }
+            }
           }
           // the output follows when the maximum has grown by more than 2^8, or a value scale is above the reference
           const float m_new = top > m + 8.f || m == NOTHING ? fmaxf(m, top) : m;
@@ -458,58 +499,87 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
             }
             m = m_new, ref = ref_new;
           }
+          // The groups take turns at what follows, tile by tile: side by side they would both wait for the exponentials and then both for the products.
+          if (ok && i > 0) ok = wait(WEIGHED + (1 - g), (others + (uint32_t)(i - 1) / 2u) & 1u);
+          if (L::P_APART && ok && !first) {  // the group's probabilities before these have been used
+            ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
           // Probabilities times share, over the scores that have been read: the share is a power of two and goes into the exponent (2^-60 at
           // least: what lies below adds nothing to a half), and the sum of a block's is brought back by it.
           const int ref_e = (int)(__float_as_uint(ref) >> 23);
-          auto weigh = [&](uint32_t(&x)[16], int b) {
-            const float ks = __shfl_sync(0xffffffffu, scale, b), vs = __shfl_sync(0xffffffffu, scale, 8 + b);
-            const int e = max((int)(__float_as_uint(vs) >> 23) - ref_e + 7, -60);
-            const float f = factor * ks, from = (float)e - m, back = __uint_as_float((uint32_t)(127 - e) << 23);
-            uint32_t packed[8];
-            if (whole) {
-              const uint64_t f2 = pair(f, f), from2 = pair(from, from);
-              uint64_t sum2 = 0ull;
+          auto weigh = [&](const uint32_t(&x)[32], int b) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int e = max(ve[b + h] - ref_e, -60);
+              const float from = (float)e - m;
+              const uint64_t f2 = pair(f[b + h], f[b + h]), from2 = pair(from, from);
+              uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
               for (int k = 0; k < 16; k += 2) {
-                const uint64_t y = fma2((uint64_t)x[k] | ((uint64_t)x[k + 1] << 32), f2, from2);
+                const uint64_t y = fma2((uint64_t)x[16 * h + k] | ((uint64_t)x[16 * h + k + 1] << 32), f2, from2);
                 const float x0 = ex2(__uint_as_float((uint32_t)y)), x1 = ex2(__uint_as_float((uint32_t)(y >> 32)));
-                sum2 = add2(sum2, pair(x0, x1));
-                packed[k / 2] = pack_half(x0, x1);
+                sum2[k / 2 & 1] = add2(sum2[k / 2 & 1], pair(x0, x1));
+                packed[8 * h + k / 2] = pack_half(x0, x1);
               }
-              l = fmaf(__uint_as_float((uint32_t)sum2) + __uint_as_float((uint32_t)(sum2 >> 32)), back, l);
-            } else {
-              float sum = 0.f;
-#pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const int key = key0 + b * BLOCK + k;
-                const float x0 = ks < 0.f || hidden(key) ? 0.f : ex2(fmaf(__uint_as_float(x[k]), f, from));
-                const float x1 = ks < 0.f || hidden(key + 1) ? 0.f : ex2(fmaf(__uint_as_float(x[k + 1]), f, from));
-                sum += x0 + x1;
-                packed[k / 2] = pack_half(x0, x1);
-              }
-              l = fmaf(sum, back, l);
+              const uint64_t both = add2(sum2[0], sum2[1]);
+              l = fmaf(__uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32)), __uint_as_float((uint32_t)(127 - e) << 23), l);
             }
-            tmem_store8(s_at + 8u * b, packed);
+            tmem_store16(p_at + 8u * b, packed);
           };
-          tc::tmem_load16(s_at, ra);
+          if (whole) {
+            tc::tmem_load32(s_at, ra);
+            tmem_wait_load(ra);
+            tc::tmem_load32(s_at + 32u, rb);
+            weigh(ra, 0);
+            tmem_wait_load(rb);
+            tc::tmem_load32(s_at + 64u, ra);
+            weigh(rb, 2);
+            tmem_wait_load(ra);
+            tc::tmem_load32(s_at + 96u, rb);
+            weigh(ra, 4);
+            tmem_wait_load(rb);
+            weigh(rb, 6);
+          } else {
 #pragma unroll 1
-          for (int b = 0; b < 8; b += 2) {
-            tmem_wait_load16(ra);
-            tc::tmem_load16(s_at + 16u * (b + 1), rb);
-            weigh(ra, b);
-            tmem_wait_load16(rb);
-            if (b < 6) tc::tmem_load16(s_at + 16u * (b + 2), ra);
-            weigh(rb, b + 1);
+            for (int b = 0; b < 8; b += 2) {
+              const float k0 = __shfl_sync(0xffffffffu, scale, b), k1 = __shfl_sync(0xffffffffu, scale, b + 1);
+              const float v0 = __shfl_sync(0xffffffffu, scale, 8 + b), v1 = __shfl_sync(0xffffffffu, scale, 9 + b);
+              uint32_t packed[16];
+              tc::tmem_load32(s_at + 16u * b, ra);
+              tmem_wait_load(ra);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float ks = h ? k1 : k0, by = factor * ks;
+                const int lo = lo_vis - (b + h) * BLOCK, hi = ks < 0.f ? 0 : hi_vis - (b + h) * BLOCK;
+                const int e = max((int)(__float_as_uint(h ? v1 : v0) >> 23) + 7 - ref_e, -60);
+                const float from = (float)e - m;
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                  float x0 = ex2(fmaf(__uint_as_float(ra[16 * h + k]), by, from)), x1 = ex2(fmaf(__uint_as_float(ra[16 * h + k + 1]), by, from));
+                  x0 = k >= lo && k < hi ? x0 : 0.f;
+                  x1 = k + 1 >= lo && k + 1 < hi ? x1 : 0.f;
+                  sum += x0 + x1;
+                  packed[8 * h + k / 2] = pack_half(x0, x1);
+                }
+                l = fmaf(sum, __uint_as_float((uint32_t)(127 - e) << 23), l);
+              }
+              tmem_store16(p_at + 8u * b, packed);
+            }
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
+        __syncwarp();
+        if (lane == 0 && ok) arrive(bar(WEIGHED + g));
         if (!whole && ok) {  // values that are NaN, of the keys that this row sees
           const uint32_t stage = (v_count + (uint32_t)i) & 1u;
           ok = wait(V_FULL + (int)stage, ((v_count + (uint32_t)i) >> 1) & 1u);
           int some = 0;
           {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) some |= reinterpret_cast<const int*>(smem + L::NAN_SOME)[stage * 4 + k];
+            for (int k = 0; k < 8; ++k) some |= reinterpret_cast<const int*>(smem + L::NAN_SOME)[stage * 8 + k];
           }
           if (ok && some) {
             const uint32_t* bits = reinterpret_cast<const uint32_t*>(smem + L::NAN_BITS) + stage * (TC_KEYS * (DH / 32));
@@ -528,6 +598,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         first = false;
       }
       v_count += (uint32_t)s.n_tiles;
+      others += (uint32_t)(s.n_tiles + g) / 2u;
       // the unit's end: both groups' outputs, each group half of the columns
       if (ok && !first) ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
       ml[g * 128 + row] = make_float4(m, l, ref, first ? 0.f : 1.f);
@@ -547,28 +618,36 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         const size_t part_row = (size_t)s.part * TC_ROWS + row;
         const size_t to = s.part < 0 ? (size_t)(s.token0 + q) * p.out_stride + (size_t)h * DH : part_row * DH;
 #pragma unroll 1
-        for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 16) {
-          uint32_t ra[16], rb[16];
-          tc::tmem_load16(o_at + (uint32_t)c, ra);
-          tc::tmem_load16(o_at + (uint32_t)(DH + c), rb);
-          tmem_wait_load16(ra);
-          tmem_wait_load16(rb);
-          float o[16];
+        for (int c = g * (DH / 2); c < (g + 1) * (DH / 2); c += 32) {
+          uint32_t ra[32], rb[32];
+          tc::tmem_load32(o_at + (uint32_t)c, ra);
+          tc::tmem_load32(o_at + (uint32_t)(DH + c), rb);
+          tmem_wait_load(ra);
+          tmem_wait_load(rb);
+          float o[32];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = (a.w != 0.f ? __uint_as_float(ra[k]) * ua : 0.f) + (b.w != 0.f ? __uint_as_float(rb[k]) * ub : 0.f);
+          for (int k = 0; k < 32; ++k) o[k] = (a.w != 0.f ? __uint_as_float(ra[k]) * ua : 0.f) + (b.w != 0.f ? __uint_as_float(rb[k]) * ub : 0.f);
           if (bad_somewhere) {
-            const uint32_t word = (bad_at[c / 32] | bad_at[128 * (DH / 32) + c / 32]) >> (c % 32);
+            const uint32_t word = bad_at[c / 32] | bad_at[128 * (DH / 32) + c / 32];
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
+            for (int k = 0; k < 32; ++k)
               if ((word >> k) & 1u) o[k] = CUDART_NAN_F;
           }
           if (row_ok) {
+            if (s.part < 0) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              if (s.part < 0)
-                store4<false>(p.out, to + c + k, o[k], o[k + 1], o[k + 2], o[k + 3]);
-              else
-                *reinterpret_cast<float4*>(p.part_o + to + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              for (int k = 0; k < 32; k += 8) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const __nv_bfloat162 x = __floats2bfloat162_rn(o[k + 2 * j], o[k + 2 * j + 1]);
+                  u[j] = *reinterpret_cast<const uint32_t*>(&x);
+                }
+                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + to + c + k) = make_uint4(u[0], u[1], u[2], u[3]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(p.part_o + to + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
             }
           }
         }
@@ -579,7 +658,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       if (lane == 0) arrive(bar(O_FREE));
       done_with(n);
     }
-  } else if (warp == 12) {
+  } else if (warp == 16) {
     // ---- products: the whole warp walks, one lane issues ----
     constexpr uint32_t idesc_s = tc_instr_desc(TC_KEYS, false), idesc_o = tc_instr_desc(DH, true);
     const uint64_t q_desc = tc::smem_desc(base + L::Q), k_desc = tc::smem_desc(base + L::K), v_desc = tc_desc_mn(base + L::V);
@@ -588,10 +667,10 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
     bool ok = true;
     for (uint32_t n = 0; ok && next_segment(n, s); ++n) {
       ok = wait(Q_READY, n & 1u);
-      auto issue_s = [&](int i) {  // scores of tile i, over the probabilities that the group's tile before has left there
+      auto issue_s = [&](int i) {  // scores of tile i, where those of the group's tile before were, or the probabilities that they became
         const int g = i & 1;
         const uint32_t stage = (count + (uint32_t)i) & 1u;
-        if (p_count[g] > 0) ok = wait(PV_DONE + g, (p_count[g] - 1u) & 1u);
+        if (!L::P_APART && p_count[g] > 0) ok = wait(PV_DONE + g, (p_count[g] - 1u) & 1u);
         if (ok) ok = wait(K_FULL + (int)stage, ((count + (uint32_t)i) >> 1) & 1u);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -613,20 +692,21 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         const uint32_t stage = (count + (uint32_t)i) & 1u;
         if (i == 0 && n > 0) ok = wait(O_FREE, (n - 1u) & 1u);
         if (ok) ok = wait(P_READY + g, p_count[g] & 1u);
+        if (L::P_APART && ok && i + 2 < s.n_tiles) issue_s(i + 2);
         if (ok) ok = wait(V_FULL + (int)stage, ((count + (uint32_t)i) >> 1) & 1u);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (tc::elect_one()) {
 #pragma unroll
           for (int k = 0; k < TC_KEYS / 16; ++k)  // 16 keys: eight columns of packed probabilities, 16 rows of values
-            mma_from_tmem(tmem + 256u + (uint32_t)(g * DH), tmem + (uint32_t)(g * 128 + k * 8), v_desc + (uint64_t)(stage * (L::MAT >> 4) + k * (2048 >> 4)), idesc_o,
+            mma_from_tmem(tmem + 256u + (uint32_t)(g * DH), tmem + L::p_col(g) + (uint32_t)(k * 8), v_desc + (uint64_t)(stage * (L::MAT >> 4) + k * (2048 >> 4)), idesc_o,
                           i >= 2 || k != 0 ? 1u : 0u);
           tc::mma_commit(bar(V_EMPTY + (int)stage));
           tc::mma_commit(bar(PV_DONE + g));
         }
         __syncwarp();
         ++p_count[g];
-        if (i + 2 < s.n_tiles) issue_s(i + 2);
+        if (!L::P_APART && i + 2 < s.n_tiles) issue_s(i + 2);
       }
       count += (uint32_t)s.n_tiles;
       done_with(n);
@@ -665,7 +745,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 template <int DH>
@@ -676,9 +756,9 @@ int launch_attention_tc(AttnParams8 p, int blocks, cudaStream_t stream) {
   const auto kernel = kv8_attention_tc_kernel<DH>;
   const int rc = (int)note_launch(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES));
   if (rc != 0) return take_launch_error();
-  p.cost = 2;
+  p.cost = 6;
   launch_pdl_split(false, kernel, dim3(blocks), dim3(TC_THREADS), L::BYTES, stream, p);
-  launch_pdl(kv8_join_kernel<false, TC_ROWS>, dim3(p.n_entries, p.n_kv_heads), dim3(128), 0, stream, p);
+  launch_pdl(kv8_join_kernel<false, TC_ROWS>, dim3(p.n_entries, p.n_kv_heads, TC_ROWS / 8), dim3(128), 0, stream, p);
   return 0;
 }
 

@@ -2139,19 +2139,19 @@ def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start,
 _KV8_PLANS: dict[tuple, tuple[int, int, int, int, int, int]] = {}
 
 
-def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, span: int) -> tuple[int, int, int, int, int, int]:
+def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, page_size: int, span: int) -> tuple[int, int, int, int, int, int]:
     """(rows of a block of threads, blocks of rows, SMs or 0, blocks of threads, ints of the plan, floats of scratch) for items of up to
     ``queries`` queries.
 
     SMs 0: every unit (an item's rows for one key/value head) has a block to itself; else all keys are shared evenly by as many blocks as stand on
     the device at once, and what lies in several is joined."""
-    key = (code, is_tiles, n_items, queries, n_heads, n_kv, dh, span)
+    key = (code, is_tiles, n_items, queries, n_heads, n_kv, dh, page_size, span)
     have = _KV8_PLANS.get(key)
     if have is not None:
         return have
     rows = queries * (n_heads // n_kv)
     block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
-    if kv8_on_tcgen05(code, rows, dh):
+    if kv8_on_tcgen05(code, rows, dh, page_size, span):
         block = 128
     row_blocks = -(-rows // block)
     entries = n_items * row_blocks
@@ -2175,11 +2175,14 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
     return have
 
 
-def kv8_on_tcgen05(code: int, rows: int, dh: int) -> bool:
-    return code == BF16 and dh in (64, 128) and rows > KV8_TC_ROWS
+def kv8_on_tcgen05(code: int, rows: int, dh: int, page_size: int, span: int) -> bool:
+    """Whether items of up to ``rows`` rows (queries times the heads of a group) run on the tcgen05 kernel (csrc/kv8_attention_tc.cuh): those that
+    fill half of its 128 rows, over contexts long enough to pay for its beginning.  Measured on B200, us, mma.sync / tcgen05: 32 heads on 8 of 128, 16
+    queries x 16 of 1000 70.8 / 54.0, x 8 of 4000 77 / 71, 8 queries x 8 of 4000 (32 rows) 40.7 / 44.7, 12 x 32 of 300 (48 rows) 36.8 / 60.7, prompts
+    of 4 x 512 75 / 62, 512 of 1024 59.8 / 41.6; 12 heads of 64, prompts of 2 x 1024 53.0 / 35.1, 8 x 256 16.4 / 24.9, one of 100 10.7 / 12.9."""
+    return code == BF16 and dh in (64, 128) and rows >= 64 and span >= 512 and page_size <= 4096
 
 
-KV8_TC_ROWS = 16
 KV8_MOST_ENTRIES = 4096  # blocks of rows whose keys are shared evenly: their numbers lie in shared memory once
 
 
@@ -2190,20 +2193,21 @@ def _kv8_by_units(dh: int, span: int) -> bool:
     return span * 2 * dh <= 256 << 10
 
 
-def _kv8_plans(code: int, n_tiles: int, max_q: int, n_decode: int, n_heads: int, n_kv: int, dh: int, span: int, window: int):
+def _kv8_plans(code: int, n_tiles: int, max_q: int, n_decode: int, n_heads: int, n_kv: int, dh: int, page_size: int, span: int, window: int):
     """The plans of a call's portions and of its decoded requests (``None``: there are none)."""
     queries = min(max(int(max_q), 1), KV8_TILE_QUERIES)
     if window > 0:
         span = min(span, window + queries)
     span = max(span, 1)
-    return (_kv8_plan(code, 1, n_tiles, queries, n_heads, n_kv, dh, span) if n_tiles else None,
-            _kv8_plan(code, 0, n_decode, 1, n_heads, n_kv, dh, span) if n_decode else None)
+    return (_kv8_plan(code, 1, n_tiles, queries, n_heads, n_kv, dh, page_size, span) if n_tiles else None,
+            _kv8_plan(code, 0, n_decode, 1, n_heads, n_kv, dh, page_size, span) if n_decode else None)
 
 
-def kv8_attention_scratch(*, dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, span: int, n_tiles: int = 0,
+def kv8_attention_scratch(*, dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, page_size: int, span: int, n_tiles: int = 0,
                           max_q: int = KV8_TILE_QUERIES, n_decode: int = 0, window: int | None = None) -> int:
     """How many floats of scratch ``kv8_attention`` needs for these sizes (0: none)."""
-    plans = _kv8_plans(F32 if dtype == torch.float32 else BF16, n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, int(span), int(window or 0))
+    plans = _kv8_plans(F32 if dtype == torch.float32 else BF16, n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, page_size,
+                       int(span), int(window or 0))
     return max((plan[5] for plan in plans if plan is not None), default=0)
 
 
@@ -2257,7 +2261,7 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     if q.shape[0] == 0:
         return
     window = int(window or 0)
-    plans = _kv8_plans(code, n_tiles, max_q, n_decode, n_heads, n_kv, dh, int(span), window)
+    plans = _kv8_plans(code, n_tiles, max_q, n_decode, n_heads, n_kv, dh, page_size, int(span), window)
     need = max((plan[5] for plan in plans if plan is not None), default=0)
     if need:
         if scratch is None:

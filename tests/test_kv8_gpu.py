@@ -299,7 +299,7 @@ def test_captured_and_longer(K):
         K.kv8_attention(q, pool, scales, a["block_table"], a["q_start"], a["kv_len"], a["slots"], into, n_heads=heads, scale=0.125, span=2100,
                         tiles=a["tiles"], n_tiles=1, max_q=6, decode_reqs=a["decode_reqs"], n_decode=2)
 
-    assert K.kv8_attention_scratch(dtype=BF16, n_heads=heads, n_kv=heads, head_dim=64, span=2100, n_tiles=1, max_q=6, n_decode=2) > 0
+    assert K.kv8_attention_scratch(dtype=BF16, n_heads=heads, n_kv=heads, head_dim=64, page_size=page, span=2100, n_tiles=1, max_q=6, n_decode=2) > 0
     a["kv_len"].copy_(torch.tensor([2100, 30, 600], dtype=torch.int32))
     go(out)
     torch.cuda.synchronize()
