@@ -16,7 +16,8 @@ class DoubleFree(RuntimeError):
 
 
 class IdAllocator:
-    """Hands out ids ``0..capacity-1``; every id is either free or held, never both."""
+    """Hands out ids ``0..capacity-1``; every id is either free or held, never both.  A held id may have several holders (``share``): it is
+    free again when the last of them has given it back."""
 
     def __init__(self, capacity: int, what: str = "id") -> None:
         if capacity <= 0:
@@ -24,7 +25,7 @@ class IdAllocator:
         self.capacity = int(capacity)
         self.what = what
         self._free = list(range(self.capacity - 1, -1, -1))  # pop() gives 0 first
-        self._held = [False] * self.capacity
+        self._holders = [0] * self.capacity
 
     @property
     def num_free(self) -> int:
@@ -35,7 +36,21 @@ class IdAllocator:
         return self.capacity - len(self._free)
 
     def is_held(self, i: int) -> bool:
-        return self._held[i]
+        return self._holders[i] > 0
+
+    def holders(self, i: int) -> int:
+        return self._holders[i]
+
+    def share(self, ids) -> None:
+        """One more holder for each of ``ids``, all of which are held."""
+        ids = list(ids)
+        for i in ids:
+            if not 0 <= i < self.capacity:
+                raise ValueError(f"{self.what} {i} out of range 0..{self.capacity - 1}")
+            if not self._holders[i]:
+                raise ValueError(f"{self.what} {i} is free: it cannot be shared")
+        for i in ids:
+            self._holders[i] += 1
 
     def alloc(self, n: int = 1) -> list[int] | None:
         """``n`` ids, or ``None`` (and nothing taken) when fewer are free."""
@@ -48,26 +63,27 @@ class IdAllocator:
         out = self._free[-n:]
         del self._free[-n:]
         out.reverse()  # the order pop() would have given
-        held = self._held
+        holders = self._holders
         for i in out:
-            held[i] = True
+            holders[i] = 1
         return out
 
     def free(self, ids) -> None:
         for i in ids:
             if not 0 <= i < self.capacity:
                 raise ValueError(f"{self.what} {i} out of range 0..{self.capacity - 1}")
-            if not self._held[i]:
+            if not self._holders[i]:
                 raise DoubleFree(f"{self.what} {i} freed while not held")
-            self._held[i] = False
-            self._free.append(i)
+            self._holders[i] -= 1
+            if not self._holders[i]:
+                self._free.append(i)
 
     def check(self) -> None:
-        """Raise if the free list and the held flags disagree."""
+        """Raise if the free list and the holders' numbers disagree."""
         if len(set(self._free)) != len(self._free):
             raise AssertionError(f"{self.what}: an id is twice on the free list")
         for i in self._free:
-            if self._held[i]:
+            if self._holders[i]:
                 raise AssertionError(f"{self.what} {i} is both free and held")
-        if sum(self._held) + len(self._free) != self.capacity:
+        if sum(1 for n in self._holders if n) + len(self._free) != self.capacity:
             raise AssertionError(f"{self.what}: an id is lost")

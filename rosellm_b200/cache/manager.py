@@ -15,7 +15,11 @@ that uses the slot.
 
 Pool layout of one layer: ``[pages, 2 (key, value), kv heads, page size, head
 dim]`` (one plane instead of two where the spec says that a token's row serves as both); the reference keeps K and V as two ``[layers, blocks, heads, 64, dim]``
-tensors (rosellm/roseinfer/engine.py:4397-4408).
+tensors (rosellm/roseinfer/engine.py:4397-4408).  A cache held in 8 bits (``eight_bits``) has codes in the pool, float8_e4m3fn, and a scale
+for every 16 tokens of a page, plane and head beside it.
+
+A request may go on as two (``fork``): the second one's block table names the first's whole pages, which neither writes any more, and a page of its
+own with a copy of the last, partly filled one.  A page is free again when the last request that holds it has given it back.
 
 All bookkeeping is on the host; device tensors are touched only by
 ``sync_to_device`` (dirty block-table rows, state resets).
@@ -39,6 +43,8 @@ class CacheGroup:
     table: np.ndarray  # int32 [slots, max_pages_per_seq]; -1 where no page is held
     first_page: np.ndarray  # int64 [slots]: lowest logical page still held (window groups)
     pools: dict[int, torch.Tensor] = field(default_factory=dict)
+    scales: dict[int, torch.Tensor] = field(default_factory=dict)  # of pools held in 8 bits
+    page_pools: object = None  # what ``copy_pages`` takes: every tensor with this group's pages
     device_table: torch.Tensor | None = None
     host_table: torch.Tensor | None = None  # tensor view of ``table``
     snapshots: list = field(default_factory=list)  # pinned copies of the table that uploads read
@@ -70,13 +76,22 @@ class CacheManager:
         dtype: torch.dtype = torch.float32,
         device: str | torch.device = "cpu",
         allocate_pools: bool = True,
+        eight_bits: bool = False,
     ) -> None:
         self.page_size = int(page_size)
         self.num_pages = int(num_pages)
         self.max_slots = int(max_slots)
         self.max_seq_len = int(max_seq_len)
         self.max_pages_per_seq = pages_for(self.max_seq_len, self.page_size)
-        self.dtype = dtype
+        self.dtype = torch.float8_e4m3fn if eight_bits else dtype
+        self.eight_bits = bool(eight_bits)
+        if self.eight_bits:
+            from ..ops.kernels import KV8_BLOCK, kv8_fits
+
+            for key, spec in kv_specs.items():
+                if spec.planes != 2 or not kv8_fits(self.page_size, spec.head_dim):
+                    raise ValueError(f"cache of layer {key}: 8 bits take keys and values of head sizes that are multiples of 32, up to 256, in pages of a "
+                                     f"multiple of {KV8_BLOCK} tokens; got {spec.planes} planes, head size {spec.head_dim}, pages of {self.page_size}")
         self.device = torch.device(device)
         self.slots = IdAllocator(self.max_slots, "slot")
         self.num_tokens = np.zeros(self.max_slots, dtype=np.int64)
@@ -101,8 +116,13 @@ class CacheManager:
                 for layer in layers:
                     group.pools[layer] = torch.zeros(
                         (self.num_pages, spec.planes, spec.num_kv_heads, self.page_size, spec.head_dim),
-                        dtype=dtype, device=self.device,
+                        dtype=self.dtype, device=self.device,
                     )
+                    if self.eight_bits:
+                        group.scales[layer] = torch.zeros(
+                            (self.num_pages, spec.planes, spec.num_kv_heads, self.page_size // KV8_BLOCK),
+                            dtype=torch.float32, device=self.device,
+                        )
                 group.device_table = torch.full(
                     (self.max_slots, self.max_pages_per_seq), -1, dtype=torch.int32,
                     device=self.device,
@@ -124,6 +144,10 @@ class CacheManager:
     # ---- what parts read -------------------------------------------------
     def kv_pool(self, layer) -> torch.Tensor:
         return self.groups[self.group_of_layer[layer]].pools[layer]
+
+    def kv_scales(self, layer) -> torch.Tensor | None:
+        """The scales of a cache held in 8 bits; ``None`` for one in the engine's own type."""
+        return self.groups[self.group_of_layer[layer]].scales.get(layer)
 
     def block_table(self, layer) -> torch.Tensor:
         return self.groups[self.group_of_layer[layer]].device_table
@@ -214,6 +238,50 @@ class CacheManager:
                 g.first_page[slot] = keep_from
                 self._dirty_rows.add(slot)
 
+    def fork(self, slot: int) -> int | None:
+        """A slot for a request that goes on from where ``slot`` stands: the same cached tokens and state, of which either's further steps
+        change nothing for the other.  Whole pages are shared; the last page, where it is partly filled, is copied, in all layers at once, on the
+        current stream (behind the steps that have been issued, ahead of those that will be).  ``None``, and nothing taken, when no slot or not
+        every page is to be had.  Pages that ``slot`` has reserved for tokens not yet committed are not among those that are shared."""
+        if not self.slots.is_held(slot):
+            raise ValueError(f"slot {slot} is not live")
+        cur = int(self.num_tokens[slot])
+        whole, rest = divmod(cur, self.page_size)
+        if self.slots.num_free < 1 or (rest and any(g.allocator.num_free < 1 for g in self.groups)):
+            return None
+        new = self.slots.alloc(1)[0]
+        self.num_tokens[new] = cur
+        for g in self.groups:
+            lo = int(g.first_page[slot])
+            g.first_page[new] = lo
+            shared = g.table[slot, lo:whole]
+            g.allocator.share(int(p) for p in shared if p >= 0)
+            g.table[new, lo:whole] = shared
+            if rest:
+                src, dst = int(g.table[slot, whole]), g.allocator.alloc(1)[0]
+                g.table[new, whole] = dst
+                self._copy_page(g, src, dst)
+        self._dirty_rows.add(new)
+        if slot in self._slots_to_reset:  # nothing has run yet: the new one's state begins from nothing as well
+            self._slots_to_reset.append(new)
+        else:
+            for t in self.states.values():
+                t[new].copy_(t[slot])
+        return new
+
+    def _copy_page(self, g: CacheGroup, src: int, dst: int) -> None:
+        if not g.pools:
+            return  # bookkeeping alone
+        if self.device.type != "cuda":
+            for t in (*g.pools.values(), *g.scales.values()):
+                t[dst].copy_(t[src])
+            return
+        from ..ops.kernels import PagePools, copy_pages
+
+        if g.page_pools is None:
+            g.page_pools = PagePools([*g.pools.values(), *g.scales.values()])
+        copy_pages(g.page_pools, torch.tensor([[src, dst]], dtype=torch.int32, device=self.device))
+
     def release(self, slot: int) -> None:
         """The request is over (finished, aborted or preempted): everything it holds goes back."""
         if not self.slots.is_held(slot):
@@ -290,24 +358,24 @@ class CacheManager:
 
     # ---- checking ----------------------------------------------------------------
     def check(self) -> None:
-        """No page lost, none held twice, tables consistent with the allocators."""
+        """No page lost, none held by more or fewer than the allocators know of, tables consistent with them."""
         self.slots.check()
         for gi, g in enumerate(self.groups):
             g.allocator.check()
-            seen: dict[int, tuple[int, int]] = {}
+            seen: dict[int, list[tuple[int, int]]] = {}
             for slot in range(self.max_slots):
                 row = g.table[slot]
                 held = [(i, int(p)) for i, p in enumerate(row) if p >= 0]
                 if held and not self.slots.is_held(slot):
                     raise AssertionError(f"group {gi}: free slot {slot} holds pages")
                 for i, p in held:
-                    if p in seen:
-                        raise AssertionError(
-                            f"group {gi}: page {p} held twice: {seen[p]} and {(slot, i)}"
-                        )
                     if not g.allocator.is_held(p):
                         raise AssertionError(f"group {gi}: page {p} in a table but free")
-                    seen[p] = (slot, i)
+                    seen.setdefault(p, []).append((slot, i))
+                    if len(seen[p]) > g.allocator.holders(p):
+                        raise AssertionError(f"group {gi}: page {p} held twice: {' and '.join(map(str, seen[p]))}")
+                    if seen[p][0][1] != i or (len(seen[p]) > 1 and (i + 1) * self.page_size > int(self.num_tokens[slot])):
+                        raise AssertionError(f"group {gi}: page {p} shared by {' and '.join(map(str, seen[p]))}, not as one whole page of the same place")
                 if self.slots.is_held(slot):
                     cur = int(self.num_tokens[slot])
                     lo = self._first_needed_page(g, cur)
@@ -316,6 +384,9 @@ class CacheManager:
                             raise AssertionError(
                                 f"group {gi}: slot {slot} with {cur} tokens lacks page {i}"
                             )
+            for p, at in seen.items():
+                if len(at) != g.allocator.holders(p):
+                    raise AssertionError(f"group {gi}: page {p} has {g.allocator.holders(p)} holders, {len(at)} in tables")
             if len(seen) != g.allocator.num_held:
                 raise AssertionError(
                     f"group {gi}: {g.allocator.num_held} pages held, {len(seen)} in tables (lost pages)"

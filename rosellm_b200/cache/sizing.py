@@ -28,10 +28,17 @@ from dataclasses import dataclass
 ELEMENT_BYTES = {"bfloat16": 2, "float32": 4}
 
 
-def kv_bytes_per_token(kv_specs, dtype: str) -> int:
+EIGHT_BIT_BLOCK = 16  # tokens that share a float32 scale, by plane and head, in a cache held in 8 bits
+
+
+def kv_bytes_per_token(kv_specs, dtype: str, eight_bits: bool = False) -> int:
     """Bytes of keys and values that one cached token takes over all layers
-    (``kv_specs``: the ``KVCacheSpec`` of every layer that writes a cache)."""
-    specs = kv_specs.values() if hasattr(kv_specs, "values") else kv_specs
+    (``kv_specs``: the ``KVCacheSpec`` of every layer that writes a cache).  ``eight_bits``: a byte an entry and the token's
+    share of the scales, rounded up."""
+    specs = list(kv_specs.values() if hasattr(kv_specs, "values") else kv_specs)
+    if eight_bits:
+        rows = [(getattr(s, "planes", 2) * s.num_kv_heads, s.head_dim) for s in specs]
+        return sum(n * dim for n, dim in rows) + -(-sum(n for n, _ in rows) * 4 // EIGHT_BIT_BLOCK)
     return sum(getattr(s, "planes", 2) * s.num_kv_heads * s.head_dim * ELEMENT_BYTES[dtype] for s in specs)
 
 

@@ -11,7 +11,7 @@ for it, there being no network and no training checkpoints here), or has random
 weights (``--random-weights CONFIG.json --seed S``).  ``--prompt-ids`` (or
 ``--prompt-ids-file``, a file of ids separated by commas or white space) gives the prompt
 as token ids, for folders without a tokenizer; ids then come out as well.  The engine's own
-options: ``--dtype`` (``bf16`` or ``fp32``; ``--no-amp`` means ``fp32``), ``--page-size``,
+options: ``--dtype`` (``bf16`` or ``fp32``; ``--no-amp`` means ``fp32``), ``--page-size``, ``--kv-cache-dtype``,
 the cache's size as ``--num-pages``, ``--kv-cache-max-tokens`` or
 ``--gpu-memory-utilization``, ``--max-num-seqs`` (the reference's ``--max-batch-size``),
 ``--max-num-batched-tokens`` and ``--prefill-chunk-size``.
@@ -56,6 +56,7 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--dtype", default=None, choices=["bf16", "bfloat16", "fp32", "float32"],
                    help="precision of the whole model (default: bf16, or fp32 with --no-amp)")
     p.add_argument("--page-size", type=int, default=16, help="tokens per cache page")
+    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"], help="fp8: keys and values in 8 bits (default: in the model's precision)")
     p.add_argument("--num-pages", type=int, default=None, help="pages the cache holds")
     p.add_argument("--kv-cache-max-tokens", type=int, default=None, help="tokens the cache holds")
     p.add_argument("--gpu-memory-utilization", type=float, default=None,
@@ -164,7 +165,7 @@ def make_engine(args):
     from .engine.llm import InferenceEngine
 
     common = dict(device=args.device, use_amp=not args.no_amp, bf16=True, dtype=args.dtype,
-                  tokenizer_name=args.tokenizer_name, page_size=args.page_size, num_pages=args.num_pages,
+                  tokenizer_name=args.tokenizer_name, page_size=args.page_size, kv_cache_dtype=args.kv_cache_dtype, num_pages=args.num_pages,
                   kv_cache_max_tokens=args.kv_cache_max_tokens, gpu_memory_utilization=args.gpu_memory_utilization,
                   max_batch_size=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
                   prefill_chunk_size=args.prefill_chunk_size, sampling_seed=args.seed)

@@ -20,10 +20,16 @@ DTYPE_NAMES = {
 }
 
 
+KV_CACHE_DTYPE_NAMES = {"auto": "auto", "fp8": "fp8", "fp8_e4m3": "fp8", "float8_e4m3fn": "fp8"}
+
+
 @dataclass(frozen=True)
 class EngineConfig:
     dtype: str = "bfloat16"
     """``bfloat16``: the serving path.  ``float32``: operands and sums in 32 bits throughout."""
+    kv_cache_dtype: str = "auto"
+    """``auto``: keys and values are cached in ``dtype``.  ``fp8``: in 8 bits, with a scale for every 16 tokens, plane and head, for models whose
+    layers all mix tokens by plain attention with heads of a multiple of 32 entries (``causal_self_attention``)."""
     page_size: int = 16
     """Tokens per cache page (the reference fixes 64, rosellm/roseinfer/engine.py:230)."""
     num_pages: int | None = None
@@ -66,8 +72,13 @@ class EngineConfig:
         if self.dtype not in DTYPE_NAMES:
             raise ConfigError(f"dtype must be one of {sorted(DTYPE_NAMES)}, got {self.dtype!r}")
         object.__setattr__(self, "dtype", DTYPE_NAMES[self.dtype])
+        if self.kv_cache_dtype not in KV_CACHE_DTYPE_NAMES:
+            raise ConfigError(f"kv_cache_dtype must be one of {sorted(KV_CACHE_DTYPE_NAMES)}, got {self.kv_cache_dtype!r}")
+        object.__setattr__(self, "kv_cache_dtype", KV_CACHE_DTYPE_NAMES[self.kv_cache_dtype])
         if self.page_size <= 0:
             raise ConfigError("page_size must be positive")
+        if self.kv_cache_dtype == "fp8" and self.page_size % 16:
+            raise ConfigError(f"kv_cache_dtype fp8: pages are of a multiple of 16 tokens, got {self.page_size}")
         for name in ("max_num_seqs", "max_num_batched_tokens", "prefill_chunk_size"):
             if getattr(self, name) <= 0:
                 raise ConfigError(f"{name} must be positive")

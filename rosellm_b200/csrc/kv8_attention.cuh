@@ -85,7 +85,7 @@ __device__ __forceinline__ Work work_of(const AttnParams8& p, int entry) {
   const int q_lo = p.is_tiles ? w.first_row / group : 0, q_hi = p.is_tiles && w.rows > 0 ? (w.first_row + w.rows - 1) / group : 0;
   if (w.token0 < 0 || w.token0 + q_hi >= p.n_tokens) w.rows = 0;  // a description that does not fit the queries
   const int lo = p.window > 0 ? max(0, w.pos0 + q_lo - p.window + 1) : 0;
-  const int hi = w.pos0 + q_hi + 1;
+  const int hi = w.slot < 0 ? 0 : w.pos0 + q_hi + 1;  // padding of a fixed-size batch sees nothing
   w.first_seen = lo / BLOCK;
   w.first_block = w.first_seen / 4 * 4;  // so that a tile lies within a page of 64 tokens or more
   w.n_blocks = hi > lo && w.rows > 0 ? (hi + BLOCK - 1) / BLOCK - w.first_block : 0;
@@ -590,7 +590,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
       if (!ok) return;
       const Rows rows{w.token0, w.pos0, w.first_row, w.rows, h};
       const int b0 = w.first_block + i0 * TB, b1 = min(w.first_block + i1 * TB, w.first_block + w.n_blocks);
-      const bool has_table = w.slot >= 0 && w.slot < p.bt_rows;
+      const bool has_table = w.slot < p.bt_rows;
       const int* table = p.block_table + (size_t)(has_table ? w.slot : 0) * p.bt_cols;
       auto look_up = [&](int b) {  // the page of block b, by this lane; -1: none, -2: not wanted
         if (b >= b1 || b < w.first_seen) return -2;

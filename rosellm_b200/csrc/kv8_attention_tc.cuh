@@ -221,7 +221,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   auto page_of = [&](const TcSegment& s, int b) {  // of block b; -1: none, -2: not wanted
     if (b < s.first_seen || b >= s.end_block) return -2;
     const int e = page_index(b);
-    return s.slot >= 0 && s.slot < p.bt_rows && e < p.bt_cols ? p.block_table[(size_t)s.slot * p.bt_cols + e] : -1;
+    return s.slot < p.bt_rows && e < p.bt_cols ? p.block_table[(size_t)s.slot * p.bt_cols + e] : -1;
   };
   // whether every row of the block of threads sees every key of a tile
   auto is_whole = [&](const TcSegment& s, int key0) {

@@ -80,6 +80,8 @@ __global__ __launch_bounds__(128) void kv8_write_kernel(WriteParams p, int group
     const int plane_head = first_plane + item % n_planes;
     const int plane = plane_head >= p.n_kv_heads ? 1 : 0, head = plane_head - plane * p.n_kv_heads;
     const int req = p.req_of_token[t], pos = p.positions[t];
+    const int slot = p.slots[req];
+    if (slot < 0) continue;  // padding
     const int end = min(p.q_start[req + 1], p.n_tokens), first = p.q_start[req];
     if (pos < 0 || pos >= p.max_pos) {
       if (lane == 0) atomicOr(p.status, RL_STATUS_BAD_POSITION);
@@ -91,8 +93,8 @@ __global__ __launch_bounds__(128) void kv8_write_kernel(WriteParams p, int group
       if (lane == 0) atomicOr(p.status, RL_STATUS_BAD_POSITION);
       n = p.max_pos - pos;
     }
-    const int slot = p.slots[req], entry = pos / p.page_size;
-    const int page = slot >= 0 && slot < p.bt_rows && entry < p.bt_cols ? p.block_table[(size_t)slot * p.bt_cols + entry] : -1;
+    const int entry = pos / p.page_size;
+    const int page = slot < p.bt_rows && entry < p.bt_cols ? p.block_table[(size_t)slot * p.bt_cols + entry] : -1;
     if (page < 0 || page >= p.n_pages) {
       if (lane == 0) atomicOr(p.status, RL_STATUS_BAD_PAGE);
       continue;

@@ -132,6 +132,18 @@ class StepContext:
     def kv_pool(self, layer) -> torch.Tensor:
         return self.cache.kv_pool(layer)
 
+    def kv_scales(self, layer) -> torch.Tensor | None:
+        """The scales of a layer's cache that is held in 8 bits; ``None`` for one in the engine's own type."""
+        return self.cache.kv_scales(layer)
+
+    @property
+    def longest_portion(self) -> int:
+        """The most tokens that a request brings to the step."""
+        got = self.extras.get("_longest_portion")
+        if got is None:
+            got = self.extras["_longest_portion"] = int(np.diff(self.host.q_start).max()) if self.n_reqs else 0
+        return got
+
     def block_table(self, layer) -> torch.Tensor:
         return self.cache.block_table(layer)
 

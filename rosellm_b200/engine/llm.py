@@ -71,6 +71,7 @@ class InferenceEngine:
         prefill_chunk_size: int = 512,
         max_position_embeddings: int | None = None,
         page_size: int = 16,
+        kv_cache_dtype: str = "auto",
         cuda_graphs: bool = True,
         capture_graphs_at_start: bool = True,
         truncate_prompt: bool = False,
@@ -88,7 +89,9 @@ class InferenceEngine:
         tokens one call late.  The generated tokens are the same either way.
         The cache's size is given by one of ``kv_cache_max_tokens``, ``kv_cache_mem_fraction``,
         ``gpu_memory_utilization`` (the reference's three, rosellm/roseinfer/engine.py:96-98, 111)
-        or ``num_pages``; by none, it holds ``max_batch_size`` whole contexts.  ``sample_in_head``:
+        or ``num_pages``; by none, it holds ``max_batch_size`` whole contexts.  ``kv_cache_dtype``: ``"fp8"`` keeps keys and values in
+        8 bits with a scale for every 16 tokens, plane and head (half or a quarter of the memory and of what a decoded token reads; ``EngineConfig`` says for
+        which models).  ``sample_in_head``:
         steps whose rows are greedy or sampled by temperature alone get their tokens chosen in
         the epilogue of the head's own product, where that product has such an epilogue (up to 16
         rows; more rows of a wide vocabulary when all of them take the arg-max), instead of
@@ -101,7 +104,7 @@ class InferenceEngine:
         if device == "cuda":
             device = "cuda:0"
         ec = EngineConfig(
-            dtype=dtype, page_size=page_size, kv_cache_tokens=kv_cache_max_tokens,
+            dtype=dtype, page_size=page_size, kv_cache_dtype=kv_cache_dtype, kv_cache_tokens=kv_cache_max_tokens,
             kv_cache_mem_fraction=kv_cache_mem_fraction, gpu_memory_utilization=gpu_memory_utilization,
             num_pages=num_pages, seed=sampling_seed,
             max_num_seqs=max_batch_size, max_num_batched_tokens=max_num_batched_tokens,
@@ -177,8 +180,26 @@ class InferenceEngine:
             self._finished_ids.append(req.request_id)
         return req.request_id
 
+    def fork_request(self, request_id, *, new_request_id: int | str | None = None, seed: int | None = None,
+                     sampling_params: SamplingParams | None = None) -> int | str:
+        """A second request that goes on from where a running one stands: the same prompt, the same tokens generated so far, the same cache (whole
+        pages are shared, the last one is copied), and a random stream of its own from here on.  ``sampling_params``: how it goes on (default: as
+        the first one does; ``max_new_tokens`` counts the tokens generated so far as well).  Raises ``ValueError`` for a request that is
+        not running (waiting, or finished), and ``OutOfPages`` when there is no slot or no page for another."""
+        req = self._requests[request_id]
+        if new_request_id is not None and new_request_id in self._requests:
+            raise ValueError(f"request {new_request_id!r} exists already")
+        if self._inflight is not None:  # the token of the step in flight is part of where the request stands
+            inflight, self._inflight = self._inflight, None
+            self._read_early = {**self._read_early, **self._resolve(inflight)}
+        new = self.scheduler.fork(req, self.runner.fork, request_id=new_request_id, seed=seed, params=sampling_params)
+        self._requests[new.request_id] = new
+        if new.status == FINISHED:
+            self._finished_ids.append(new.request_id)
+        return new.request_id
+
     def has_unfinished(self) -> bool:
-        return self.scheduler.has_unfinished() or self._inflight is not None
+        return self.scheduler.has_unfinished() or self._inflight is not None or bool(self._read_early)
 
     def _launch(self, plan):
         """Enqueue the plan's step and its sampling; returns (requests that sample, token handle)."""
@@ -215,6 +236,7 @@ class InferenceEngine:
         # a request that had finished before this token arrived does not report it
         return {r.request_id: t for r, t in zip(sampling, tokens) if before[id(r)] != FINISHED}
 
+    _read_early: dict = {}  # tokens read before the call of ``step`` that reports them (replaced, never changed)
     STATUS_CHECK_EVERY = 256  # steps between two looks at the kernels' status word while requests keep coming
 
     def step(self) -> dict[int | str, int]:
@@ -227,6 +249,8 @@ class InferenceEngine:
         that never runs dry: a raised ``KernelError`` means that tokens since the last check
         may be wrong."""
         out = self._step()
+        if self._read_early:
+            out, self._read_early = {**self._read_early, **out}, {}
         self._since_status_check += 1
         if not self.has_unfinished() or self._since_status_check >= self.STATUS_CHECK_EVERY:
             self._since_status_check = 0

@@ -26,7 +26,7 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..cache.sizing import kv_bytes_per_token, plan_cache
-from ..config.base import ModelConfig, load_config, resolve_architecture
+from ..config.base import ConfigError, ModelConfig, load_config, resolve_architecture
 from ..config.engine import EngineConfig
 from ..models.model import Model
 from ..ops import kernels as K
@@ -107,6 +107,12 @@ class ModelRunner:
         self.model = Model(self.spec, self.dtype, self.device)
         self.model.load_tensors(file_tensors, source)
         kv_specs, state_specs = self.model.kv_specs(), self.model.state_specs()
+        eight_bits = ec.kv_cache_dtype == "fp8"
+        if eight_bits:
+            for i, layer in enumerate(self.model.layers):
+                for name, part in layer.parts.items():
+                    if part.cache_spec() is not None and not getattr(part, "takes_8bit_cache", False):
+                        raise ConfigError(f"kv_cache_dtype fp8: {name!r} of layer {i} ({part.kind}) keeps its cache in the engine's own type alone")
         longest = min(ec.max_model_len or self.spec.max_positions, self.spec.max_positions)
         pool_tokens = ec.kv_cache_tokens
         if (ec.num_pages is None and pool_tokens is None and ec.gpu_memory_utilization is None
@@ -118,7 +124,7 @@ class ModelRunner:
         self.cache_plan = plan = plan_cache(
             page_size=ec.page_size, max_num_seqs=ec.max_num_seqs,
             max_model_len=longest,
-            bytes_per_token=kv_bytes_per_token(kv_specs, ec.dtype),
+            bytes_per_token=kv_bytes_per_token(kv_specs, ec.dtype, eight_bits),
             num_pages=ec.num_pages, kv_cache_tokens=pool_tokens,
             gpu_memory_utilization=ec.gpu_memory_utilization, kv_cache_mem_fraction=ec.kv_cache_mem_fraction,
             mem_get_info=lambda: torch.cuda.mem_get_info(self.device),
@@ -133,7 +139,7 @@ class ModelRunner:
         self.cache = CacheManager(
             kv_specs, state_specs,
             page_size=ec.page_size, num_pages=plan.num_pages, max_slots=ec.max_num_seqs,
-            max_seq_len=self.max_model_len, dtype=self.dtype, device=self.device,
+            max_seq_len=self.max_model_len, dtype=self.dtype, device=self.device, eight_bits=eight_bits,
         )
         self.workspace = Workspace(self.device)
         t_cap, r_cap = ec.max_num_batched_tokens, ec.max_num_seqs
@@ -512,6 +518,15 @@ class ModelRunner:
         self.graph_launches += n_kernels
         self.graph_replays += 1
         return logits[:n] if logits is not None else None
+
+    def fork(self, slot: int) -> int:
+        """A slot for a request that goes on from where ``slot`` stands (``CacheManager.fork``); raises ``OutOfPages``, and takes nothing, when there is
+        no slot or no page for it."""
+        new = self.cache.fork(slot)
+        if new is None:
+            raise OutOfPages(f"no slot or no page for a second request from slot {slot} ({self.cache.num_free_slots} slots, "
+                             f"{self.cache.num_free_pages} pages free)")
+        return new
 
     def check_status(self) -> None:
         """Wait for the device and raise if a kernel flagged bad indices during earlier steps."""

@@ -160,6 +160,39 @@ class Scheduler:
         self.waiting.append(req)
         return req
 
+    def fork(self, req: Request, fork_slot, *, request_id: int | str | None = None, seed: int | None = None,
+             params: SamplingParams | None = None) -> Request:
+        """A request that goes on from where ``req`` stands, running, none of whose tokens is still unread.  ``fork_slot``: makes a slot of the
+        first one's (``ModelRunner.fork``)."""
+        if req.status != RUNNING or PENDING in req.output_ids:
+            raise ValueError(f"request {req.request_id!r} is {req.status}: only one that runs, and whose tokens have been read, can be forked")
+        if len(self.running) >= self.max_num_seqs:
+            raise ValueError(f"{len(self.running)} requests are running; at most {self.max_num_seqs}")
+        if seed is None and params is not None:
+            seed = params.seed
+        params = params if params is not None else req.params
+        if request_id is None:
+            request_id = self._next_id
+        room = self.max_model_len - len(req.prompt_ids)
+        max_new = min(params.max_new_tokens, room)
+        most = len(req.prompt_ids) + max_new - 1
+        if any(n > self.cache.num_pages for n in self._pages_to_hold(most)):
+            raise ValueError(f"request of up to {most} cached tokens can never fit the cache of {self.cache.num_pages} pages of {self.cache.page_size} tokens")
+        if seed is None:
+            seed = self.default_seed(request_id, len(req.prompt_ids))
+        new = Request(request_id, req.prompt_ids, params, seed, max_new, output_ids=list(req.output_ids), num_computed=req.num_computed)
+        if max_new <= len(new.output_ids):
+            new.status, new.finish_reason = FINISHED, "length"
+            self.finished.append(new)
+        else:
+            new.slot = fork_slot(req.slot)
+            new.status = RUNNING
+            new.admitted_at = self._admissions
+            self._admissions += 1
+            self.running.append(new)
+        self._next_id += 1
+        return new
+
     def default_seed(self, request_id: int | str, prompt_len: int) -> int:
         """The seed of a request that brings none: a checksum of the engine's seed, the
         request's id and its prompt's length, the same in every process (Python's own ``hash``

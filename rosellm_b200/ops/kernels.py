@@ -2106,7 +2106,7 @@ def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start,
 
     ``k``, ``v`` [tokens, kv heads * head dim], both float32 or both bfloat16 (views with a row stride, as the columns of a packed
     product); token t is at position ``positions[t]`` of request ``req_of_token[t]``, whose cache pages are row
-    ``slots[request]`` of ``block_table``; a request's tokens are consecutive, from ``q_start[request]`` on, at consecutive positions, and
+    ``slots[request]`` of ``block_table``; a request's tokens are consecutive, from ``q_start[request]`` on, at consecutive positions,
     no two requests share a page that the step writes.  A block of 16 tokens gets the smallest power of two s as its scale with which
     all that the step brings into it is at most 448 s; a block that holds earlier tokens of the request keeps its scale if that is larger, and
     where it is not, the earlier codes are brought to the new one.  An infinity or NaN is stored as NaN and does not count for the scale.
@@ -2203,6 +2203,12 @@ def _kv8_plans(code: int, n_tiles: int, max_q: int, n_decode: int, n_heads: int,
             _kv8_plan(code, 0, n_decode, 1, n_heads, n_kv, dh, page_size, span) if n_decode else None)
 
 
+def kv8_attention_plan(*, dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, page_size: int, span: int, n_tiles: int = 0,
+                       max_q: int = KV8_TILE_QUERIES, n_decode: int = 0, window: int | None = None) -> tuple:
+    """What ``kv8_attention`` launches for these sizes, as a value to compare: calls of equal sizes and equal plans make the same launches."""
+    return _kv8_plans(F32 if dtype == torch.float32 else BF16, n_tiles, max_q, n_decode, n_heads, n_kv, head_dim, page_size, int(span), int(window or 0))
+
+
 def kv8_attention_scratch(*, dtype: torch.dtype, n_heads: int, n_kv: int, head_dim: int, page_size: int, span: int, n_tiles: int = 0,
                           max_q: int = KV8_TILE_QUERIES, n_decode: int = 0, window: int | None = None) -> int:
     """How many floats of scratch ``kv8_attention`` needs for these sizes (0: none)."""
@@ -2220,7 +2226,8 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     ``q`` [tokens, heads * head dim] float32 or bfloat16 (a view with a row stride), ``out`` the same shape and type (rows at multiples of
     16 bytes).  ``tiles`` int32 [n_tiles, 2]: (request, first query) of every 64 queries of the requests that bring several (``max_q``: the most
     that one of them brings), ``decode_reqs`` int32 [n_decode]: the requests that bring one.  Rows of ``out`` that belong to
-    neither are left as they are.  A query without a key in sight (``kv_len`` 0, or pages missing, which sets the status word) gets zeros.
+    neither are left as they are.  A query without a key in sight (``kv_len`` 0, a negative slot, which is padding, or pages missing, which sets the
+    status word) gets zeros.
     ``span``: the longest context of these requests; it decides how their keys are shared out over blocks, not which keys
     are seen (a captured call serves longer contexts too).  ``scratch``: float32, ``kv8_attention_scratch`` entries, for results of
     shares of the keys; none given, it is allocated for the call (a call that is being recorded has to bring its own).  Calls that may run

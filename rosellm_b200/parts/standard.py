@@ -358,6 +358,7 @@ class CausalSelfAttention(Part):
     graph_safe = True
     launches_replayable = True
     takes_norm_input = True  # h may be a K.NormInput: the qkv product then normalises its own input
+    takes_8bit_cache = True  # its pools may hold codes, with scales beside them (csrc/kv8.cuh)
     keeps_fused_weights = True  # as in DenseMLP
 
     def __init__(self, hidden_size: int, num_heads: int, head_dim: int, num_kv_heads: int | None = None,
@@ -505,6 +506,8 @@ class CausalSelfAttention(Part):
     def launch_key(self, ctx) -> tuple:
         """The longest context decides how decoded requests are split over blocks, how many warps those have and whether they are clusters,
         and which kernel takes the prompt portions."""
+        if self._eight_bits(ctx):
+            return self._plan8(ctx)
         plan = ctx.extras.get("decode_plan") or self.decode_plan(ctx) if ctx.n_decode else None
         return (plan, plan and self._decode_in_cluster(ctx, *plan), self.decode_sixteen_for(plan[0], self._decode_span(ctx), ctx.act_dtype) if plan else None,
                 self._tc_prompt_attention(ctx) if ctx.n_tiles else None)
@@ -524,7 +527,7 @@ class CausalSelfAttention(Part):
         """A step of few decoded requests and nothing else: the whole of this part (its norm
         included) can be one kernel, where the sizes fit."""
         n = ctx.n_tokens
-        return (self._out_weight_packed is not None and K.FUSED_ROWS and n <= 16
+        return (self._out_weight_packed is not None and K.FUSED_ROWS and n <= 16 and not self._eight_bits(ctx)
                 and isinstance(h, K.NormInput) and h.x is x and n == ctx.n_decode == ctx.n_reqs and run.writes_cache
                 and not getattr(ctx.position, "rotates", True))
 
@@ -533,6 +536,9 @@ class CausalSelfAttention(Part):
             K.attn_block_fused(x, h, self.qkv_weight, self.qkv_bias, self._out_weight_packed, self.out_bias,
                                ctx.kv_pool(run.cache_key), ctx.block_table(run.cache_key), ctx.positions, ctx.slots,
                                n_heads=self.num_heads, scale=self.scale, max_pos=ctx.cache.max_seq_len)
+            return
+        if self._eight_bits(ctx):
+            self._forward8(ctx, run, h, x, add)
             return
         n = ctx.n_tokens
         qkv_w = self.q_width + 2 * self.kv_width
@@ -574,6 +580,38 @@ class CausalSelfAttention(Part):
                     # prompt portions: the tcgen05 kernel (where its sizes fit) wins once a block
                     # walks several tiles of keys; short contexts are faster on mma.sync
                     prefill_path=None if self._tc_prompt_attention(ctx) else "mma")
+        K.linear(o, self.out_weight, self.out_bias, x, residual=add)
+
+
+    @staticmethod
+    def _eight_bits(ctx) -> bool:
+        return getattr(getattr(ctx, "cache", None), "eight_bits", False)
+
+    def _sizes8(self, ctx) -> dict:
+        return dict(n_heads=self.num_heads, span=self._decode_span(ctx), window=self.window, n_tiles=ctx.n_tiles_wide, max_q=ctx.longest_portion,
+                    n_decode=ctx.n_decode)
+
+    def _plan8(self, ctx) -> tuple:
+        return K.kv8_attention_plan(dtype=ctx.act_dtype, n_kv=self.num_kv_heads, head_dim=self.head_dim, page_size=ctx.cache.page_size, **self._sizes8(ctx))
+
+    def _forward8(self, ctx, run, h, x, add: bool) -> None:
+        """``forward`` over a cache held in 8 bits: keys and values leave the product as they are, for the write that rounds them."""
+        n = ctx.n_tokens
+        qkv = ctx.workspace.get("qkv", (n, self.q_width + 2 * self.kv_width), ctx.act_dtype)
+        pool, scales, table = ctx.kv_pool(run.cache_key), ctx.kv_scales(run.cache_key), ctx.block_table(run.cache_key)
+        K.linear(h, self.qkv_weight, self.qkv_bias, qkv)
+        if self._split[0] is not qkv:
+            self._split = (qkv, qkv[:, : self.q_width], qkv[:, self.q_width: self.q_width + self.kv_width],
+                           qkv[:, self.q_width + self.kv_width:])
+        _, q, k, v = self._split
+        ctx.position.rotate(ctx, q, k)
+        if run.writes_cache:
+            K.kv8_write(k, v, pool, scales, table, ctx.positions, ctx.req_of_token, ctx.q_start, ctx.slots, ctx.cache.max_seq_len)
+        o = ctx.workspace.get("attn_out", (n, self.q_width), ctx.act_dtype)
+        sizes = self._sizes8(ctx)
+        floats = K.kv8_attention_scratch(dtype=ctx.act_dtype, n_kv=self.num_kv_heads, head_dim=self.head_dim, page_size=ctx.cache.page_size, **sizes)
+        K.kv8_attention(q, pool, scales, table, ctx.q_start, ctx.kv_len, ctx.slots, o, scale=self.scale, tiles=ctx.tiles_wide,
+                        decode_reqs=ctx.decode_reqs, scratch=ctx.workspace.get("kv8_scratch", (floats,), torch.float32) if floats else None, **sizes)
         K.linear(o, self.out_weight, self.out_bias, x, residual=add)
 
 

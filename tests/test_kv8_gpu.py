@@ -252,6 +252,36 @@ def test_rows_of_no_item_stay(K):
     assert (out[:7] == 7).all() and (out[8:] == 7).all() and not (out[7] == 7).any()
 
 
+@pytest.mark.parametrize("each", [[(30, 1), (40, 1), (20, 1), (1, 1)], [(600, 64), (90, 1), (700, 100), (20, 1)]])
+def test_padding(K, each):
+    """Requests in negative slots, as a batch of a fixed size is filled up with: nothing is written for them, their rows of the output are zeros,
+    the others are as they would be, and the status word stays clear."""
+    batch = P.Batch(each, 16)
+    gen = torch.Generator().manual_seed(6)
+    pool, scales = (t.to(DEV) for t in cache_of(batch, 2, 64, gen))
+    k, v = (x.to(DEV) for x in packed(batch, 2, 64, BF16, gen))
+    q = torch.randn(batch.tokens, 256, generator=gen).to(BF16).to(DEV)
+    slots = list(batch.slots)
+    batch.slots = [slots[0], -1, -5, slots[3]]
+    before = pool.view(torch.uint8).clone(), scales.clone()
+    do_write(K, batch, k, v, pool, scales)
+    out = do_attention(K, batch, q, pool, scales, 4)
+    K.check_status(DEV)
+    rows = [slice(batch.q_start[r], batch.q_start[r + 1]) for r in range(4)]
+    assert (out[rows[1]] == 0).all() and (out[rows[2]] == 0).all()
+    for r in (1, 2):
+        pages = [p for p in batch.table[slots[r]].tolist() if p >= 0]
+        assert pool.view(torch.uint8)[pages].equal(before[0][pages]) and scales[pages].equal(before[1][pages])
+    batch.slots = slots
+    alone_pool, alone_scales = before[0].clone().view(torch.float8_e4m3fn), before[1].clone()
+    do_write(K, batch, k, v, alone_pool, alone_scales)
+    want, rough, fine = P.attention(batch, q.cpu().double().unflatten(1, (4, 64)), P.values_of(alone_pool), alone_scales.cpu().double(), 4, 64 ** -0.5)
+    for r in (0, 3):
+        pages = [p for p in batch.table[slots[r]].tolist() if p >= 0]
+        assert pool.view(torch.uint8)[pages].equal(alone_pool.view(torch.uint8)[pages]) and scales[pages].equal(alone_scales[pages])
+        compare(out[rows[r]], want[rows[r]], rough[rows[r]], fine[rows[r]], BF16)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_no_key_in_sight(K, dtype):
     """A request without keys, and one whose pages are missing: zeros, and the status word for the second."""
