@@ -30,10 +30,8 @@ __device__ __forceinline__ float scale_for(float a) {
 // 1 / s for a power of two from 2^-126 to 2^126.
 __device__ __forceinline__ float inverse_of(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// Two floats to two codes, nearest, ties to even; `lo` in the low byte.  Infinities become NaN, as NaN does.
+// Two floats to two codes, nearest, ties to even; `lo` in the low byte.  NaN stays NaN; an infinity would become 448, and is turned into NaN before.
 __device__ __forceinline__ uint16_t encode2(float lo, float hi) {
-  lo = fabsf(lo) <= 3.4e38f ? lo : CUDART_NAN_F;
-  hi = fabsf(hi) <= 3.4e38f ? hi : CUDART_NAN_F;
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;

@@ -2077,28 +2077,79 @@ def kv8_fits(page_size: int, head_dim: int) -> bool:
     return page_size > 0 and page_size % KV8_BLOCK == 0 and 0 < head_dim <= 256 and head_dim % 32 == 0
 
 
-def _kv8_pool(pool, scales, what: str) -> tuple[int, int, int, int]:
-    """(pages, kv heads, page size, head dim) of a checked 8-bit cache."""
-    if pool.dim() != 5 or pool.shape[1] != 2:
+# The checks below come at every call, of which a decoded token makes one a layer: each asks a tensor once, and which of several tensors is at
+# fault is found out only when one is.  (B200's host, a call that launches one kernel: 17.7 us with the checks tensor by tensor, 13.9 so.)
+
+def _kv8_pool(pool, scales, what: str) -> tuple[int, int, int, int, int, int]:
+    """(the current device, the pool's address, pages, kv heads, page size, head dim) of a checked 8-bit cache on that device."""
+    shape = pool.shape
+    if len(shape) != 5 or shape[1] != 2:
         raise KernelError(f"{what}: the pool must be [pages, 2, kv heads, page size, head dim]")
-    _need(pool, "pool", torch.float8_e4m3fn)
-    _need(scales, "scales", torch.float32)
-    n_pages, _, n_kv, page_size, dh = pool.shape
+    if not pool.is_cuda:
+        _need(pool, "pool")
+    here = torch.cuda.current_device()
+    if (pool.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32 or pool.get_device() != here or scales.get_device() != here
+            or not pool.is_contiguous() or not scales.is_contiguous()):
+        _need(pool, "pool", torch.float8_e4m3fn)
+        _need(scales, "scales", torch.float32)
+        _on_current_device(what, here, pool, scales)
+    n_pages, _, n_kv, page_size, dh = shape
     if not kv8_fits(page_size, dh):
         raise KernelError(f"{what}: page size {page_size} must be a multiple of {KV8_BLOCK} and head size {dh} one of 32, up to 256")
-    if tuple(scales.shape) != (n_pages, 2, n_kv, page_size // KV8_BLOCK):
+    if scales.shape != (n_pages, 2, n_kv, page_size // KV8_BLOCK):
         raise KernelError(f"{what}: scales must be [pages, 2, kv heads, page size / {KV8_BLOCK}]")
-    if pool.data_ptr() % 16:
+    at = pool.data_ptr()
+    if at % 16:
         raise KernelError(f"{what}: the pool must begin at a multiple of 16 bytes")
-    return n_pages, n_kv, page_size, dh
+    return here, at, n_pages, n_kv, page_size, dh
 
 
-def _on_current_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+def _kv8_rows(what: str, names: tuple[str, str], x, y, width: int, here: int) -> tuple[int, int, int, int, int, int, int]:
+    """(element code, rows, stride and address of x, the same of y) of two tensors of one type on the current device, rows of ``width`` entries at
+    multiples of 16 bytes."""
+    code = _code(x)
+    if y.dtype is not x.dtype or x.get_device() != here or y.get_device() != here:
+        _need(x, names[0], contiguous=False)
+        _need(y, names[1], x.dtype, contiguous=False)
+        _on_current_device(what, here, x, y)
+    xs, ys, xt, yt = x.shape, y.shape, x.stride(), y.stride()
+    if len(xs) != 2 or len(ys) != 2 or xs[1] != width or ys[1] != width or xt[1] != 1 or yt[1] != 1:
+        raise KernelError(f"{what}: {names[0]} and {names[1]} must be rows of heads * head size entries, {width}")
+    xa, ya = x.data_ptr(), y.data_ptr()
+    if (xa | ya) % 16 or (xt[0] | yt[0]) % (4 if code == F32 else 8):
+        raise KernelError(f"{what}: rows of {names[0]} and {names[1]} must begin at multiples of 16 bytes")
+    return code, xs[0], xt[0], xa, ys[0], yt[0], ya
+
+
+def _kv8_ints(here: int, names: str, *tensors) -> None:
+    """Contiguous int32 tensors on the current device."""
+    for i, t in enumerate(tensors):
+        if t.dtype is not torch.int32 or t.get_device() != here or not t.is_contiguous():
+            name = names.split()[i]
+            _need(t, name, torch.int32)
+            _on_current_device(name, here, t)
+
+
+def _on_current_device(what: str, here: int, *tensors: torch.Tensor) -> None:
     """Kernels are launched on the current device's stream: every tensor has to live there."""
-    here = torch.cuda.current_device()
-    for t in (first, *others):
-        if t is not None and t.get_device() != here:
+    for t in tensors:
+        if t.get_device() != here:
             raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{here}")
+
+
+def _stream_of(here: int) -> int:
+    return _raw_stream(here) if _raw_stream is not None else _stream()
+
+
+_status_at: dict[int, int] = {}
+
+
+def _status_address(here: int) -> int:
+    """Of the current device's status word, which stays where it is."""
+    at = _status_at.get(here)
+    if at is None:
+        at = _status_at[here] = status_word(torch.device("cuda", here)).data_ptr()
+    return at
 
 
 def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start, slots, max_pos: int) -> None:
@@ -2112,27 +2163,22 @@ def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start,
     where it is not, the earlier codes are brought to the new one.  An infinity or NaN is stored as NaN and does not count for the scale.
     Nothing else of the cache changes.  A position outside 0 .. max_pos - 1 or a block table without a page sets the status word, and the
     tokens concerned are not written."""
-    n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_write")
-    _need(k, "k", contiguous=False)
-    _need(v, "v", k.dtype, contiguous=False)
-    code = _code(k)
-    n = positions.numel()
-    for x in (k, v):
-        if x.dim() != 2 or x.shape[0] < n or x.shape[1] != n_kv * dh or x.stride(1) != 1:
-            raise KernelError("kv8_write: k and v must be rows of kv heads * head size entries, one a token")
-        if x.data_ptr() % 16 or (x.stride(0) * x.element_size()) % 16:
-            raise KernelError("kv8_write: rows of k and v must begin at multiples of 16 bytes")
-    for t, name in ((block_table, "block_table"), (positions, "positions"), (req_of_token, "req_of_token"), (q_start, "q_start"), (slots, "slots")):
-        _need(t, name, torch.int32)
-    if block_table.dim() != 2 or req_of_token.numel() < n:
+    here, pool_at, n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_write")
+    code, rows, k_stride, k_at, v_rows, v_stride, v_at = _kv8_rows("kv8_write", ("k", "v"), k, v, n_kv * dh, here)
+    _kv8_ints(here, "block_table positions req_of_token q_start slots", block_table, positions, req_of_token, q_start, slots)
+    n, table = positions.numel(), block_table.shape
+    if rows < n or v_rows < n:
+        raise KernelError("kv8_write: fewer rows of k or v than positions")
+    if len(table) != 2 or req_of_token.numel() < n:
         raise KernelError("kv8_write: block_table must be [slots, pages], and req_of_token as long as positions")
-    _on_current_device("kv8_write", pool, scales, k, v, block_table, positions, req_of_token, q_start, slots)
+    n_reqs = q_start.numel() - 1
+    if n_reqs < 0 or slots.numel() < n_reqs:
+        raise KernelError("kv8_write: q_start must be one longer than there are requests, and slots as long")
     if n == 0:
         return
-    rc = _lib().rl_kv8_write(code, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), pool.data_ptr(), scales.data_ptr(),
-                             block_table.data_ptr(), block_table.shape[0], block_table.shape[1], positions.data_ptr(), req_of_token.data_ptr(),
-                             q_start.data_ptr(), slots.data_ptr(), n, q_start.numel() - 1, n_kv, dh, page_size, n_pages, int(max_pos),
-                             status_word(pool.device).data_ptr(), _stream())
+    rc = _lib().rl_kv8_write(code, k_at, k_stride, v_at, v_stride, pool_at, scales.data_ptr(), block_table.data_ptr(), table[0],
+                             table[1], positions.data_ptr(), req_of_token.data_ptr(), q_start.data_ptr(), slots.data_ptr(), n, n_reqs, n_kv, dh,
+                             page_size, n_pages, int(max_pos), _status_address(here), _stream_of(here))
     _ok(rc, "kv8_write")
 
 
@@ -2232,65 +2278,61 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     are seen (a captured call serves longer contexts too).  ``scratch``: float32, ``kv8_attention_scratch`` entries, for results of
     shares of the keys; none given, it is allocated for the call (a call that is being recorded has to bring its own).  Calls that may run
     at the same time need scratch of their own."""
-    n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_attention")
-    _need(q, "q", contiguous=False)
-    _need(out, "out", q.dtype, contiguous=False)
-    code = _code(q)
+    global _launches
+    here, pool_at, n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_attention")
     if n_heads <= 0 or n_heads % n_kv != 0:
         raise KernelError(f"kv8_attention: {n_heads} heads are not a multiple of {n_kv} key/value heads")
-    for x, name in ((q, "q"), (out, "out")):
-        if x.dim() != 2 or x.shape[1] != n_heads * dh or x.stride(1) != 1:
-            raise KernelError(f"kv8_attention: {name} must be rows of heads * head size entries")
-        if x.data_ptr() % 16 or (x.stride(0) * x.element_size()) % 16:
-            raise KernelError(f"kv8_attention: rows of {name} must begin at multiples of 16 bytes")
-    if out.shape[0] < q.shape[0]:
+    code, n_tokens, q_stride, q_at, out_rows, out_stride, out_at = _kv8_rows("kv8_attention", ("q", "out"), q, out, n_heads * dh, here)
+    if out_rows < n_tokens:
         raise KernelError("kv8_attention: out has fewer rows than q")
-    for t, name in ((block_table, "block_table"), (q_start, "q_start"), (kv_len, "kv_len"), (slots, "slots")):
-        _need(t, name, torch.int32)
-    if block_table.dim() != 2:
-        raise KernelError("kv8_attention: block_table must be [slots, pages]")
+    _kv8_ints(here, "block_table q_start kv_len slots", block_table, q_start, kv_len, slots)
+    table = block_table.shape
+    n_reqs = q_start.numel() - 1
+    if len(table) != 2 or kv_len.numel() < n_reqs or slots.numel() < n_reqs:
+        raise KernelError("kv8_attention: block_table must be [slots, pages], q_start one longer than there are requests, kv_len and slots as long")
     if n_tiles > 0:
         if tiles is None:
             raise KernelError("kv8_attention: n_tiles without tiles")
-        _need(tiles, "tiles", torch.int32)
+        _kv8_ints(here, "tiles", tiles)
         if tiles.numel() < 2 * n_tiles:
             raise KernelError("kv8_attention: tiles is shorter than n_tiles")
     if n_decode > 0:
         if decode_reqs is None:
             raise KernelError("kv8_attention: n_decode without decode_reqs")
-        _need(decode_reqs, "decode_reqs", torch.int32)
+        _kv8_ints(here, "decode_reqs", decode_reqs)
         if decode_reqs.numel() < n_decode:
             raise KernelError("kv8_attention: decode_reqs is shorter than n_decode")
     if window is not None and window <= 0:
         raise KernelError("kv8_attention: a window sees at least one key")
-    _on_current_device("kv8_attention", pool, scales, q, out, block_table, q_start, kv_len, slots,
-                       tiles if n_tiles > 0 else None, decode_reqs if n_decode > 0 else None, scratch)
-    if q.shape[0] == 0:
+    if n_tokens == 0:
         return
     window = int(window or 0)
     plans = _kv8_plans(code, n_tiles, max_q, n_decode, n_heads, n_kv, dh, page_size, int(span), window)
-    need = max((plan[5] for plan in plans if plan is not None), default=0)
+    need = max([plan[5] for plan in plans if plan is not None], default=0)
+    at = 0
     if need:
         if scratch is None:
             if _recorder is not None:
                 raise KernelError("kv8_attention: a recorded call needs scratch that outlives it")
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-        _need(scratch, "scratch", torch.float32)
-        if scratch.numel() < need or scratch.data_ptr() % 16:
+        else:
+            _need(scratch, "scratch", torch.float32)
+            _on_current_device("kv8_attention", here, scratch)
+        at = scratch.data_ptr()
+        if scratch.numel() < need or at % 16:
             raise KernelError(f"kv8_attention: scratch of {need} floats at a multiple of 16 bytes is needed")
     lib = _lib()
     for plan, items, n_items, is_tiles in ((plans[0], tiles, n_tiles, 1), (plans[1], decode_reqs, n_decode, 0)):
         if plan is None:
             continue
         block, row_blocks, sms, at_once, ints, _ = plan
-        at = scratch.data_ptr() if sms else 0
-        made = lib.rl_launches_made()
-        rc = lib.rl_kv8_attention(code, q.data_ptr(), q.stride(0), pool.data_ptr(), scales.data_ptr(), block_table.data_ptr(),
-                                  block_table.shape[0], block_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(), slots.data_ptr(),
-                                  out.data_ptr(), out.stride(0), items.data_ptr(), n_items, is_tiles, q.shape[0], n_heads, n_kv, dh,
-                                  page_size, n_pages, window, float(scale), block, row_blocks, sms, at_once, at, at + 4 * ints,
-                                  at + 4 * (ints + at_once * 2 * block * dh), status_word(q.device).data_ptr(), _stream())
-        _ok(rc, "kv8_attention", made)
+        rc = lib.rl_kv8_attention(code, q_at, q_stride, pool_at, scales.data_ptr(), block_table.data_ptr(), table[0], table[1],
+                                  q_start.data_ptr(), kv_len.data_ptr(), slots.data_ptr(), out_at, out_stride, items.data_ptr(), n_items,
+                                  is_tiles, n_tokens, n_heads, n_kv, dh, page_size, n_pages, window, scale, block, row_blocks, sms, at_once, at,
+                                  at + 4 * ints, at + 4 * (ints + at_once * 2 * block * dh), _status_address(here), _stream_of(here))
+        _ok(rc, "kv8_attention")
+        if sms:
+            _launches += 1  # the joining of shares
 
 
 # ---- copies of cache pages -----------------------------------------------------------------------
@@ -2324,11 +2366,12 @@ def copy_pages(pools: PagePools, pairs) -> None:
     _need(pairs, "pairs", torch.int32)
     if pairs.dim() != 2 or pairs.shape[1] != 2:
         raise KernelError("copy_pages: pairs must be [n, 2]")
-    _on_current_device("copy_pages", pools.pools[0], pairs)
+    here = torch.cuda.current_device()
+    _on_current_device("copy_pages", here, pools.pools[0], pairs)
     if pairs.shape[0] == 0:
         return
     lib = _lib()
     made = lib.rl_launches_made()
     rc = lib.rl_copy_pages(pools.bases, pools.page_bytes, len(pools.pools), pairs.data_ptr(), pairs.shape[0], pools.n_pages,
-                           status_word(pairs.device).data_ptr(), _stream())
+                           _status_address(here), _stream_of(here))
     _ok(rc, "copy_pages", made)
