@@ -193,74 +193,72 @@ __global__ __launch_bounds__(128, WriteShape<T, DH>::AT_ONCE) void kv8_write_ker
     int stage = 0;
 #pragma unroll 1
     for (int plane_head = first_plane; plane_head < end_plane; plane_head += 4) {
-    fetch(plane_head + 4 * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    Piece<T> x[PASSES];
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = i * ROWS + row_in_pass;
-      if (row_in_pass < ROWS && r < n)
-        x[i].load(ring + stage * S::STAGE + i * PIECE);
-      else
-        x[i].clear();
-    }
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    const size_t page_head = (size_t)page * 2 * p.n_kv_heads + plane_head;
-    uint8_t* dst = p.pool + (page_head * p.page_size + row) * DH + col;  // of the first new token
-    float* scale_at = p.scales + page_head * (p.page_size / BLOCK) + row / BLOCK;
-    const float s_old = continued ? *scale_at : 0.f;
-    uint32_t tops = 0;
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) tops = x[i].top(tops);
-    float top = Piece<T>::top_of(tops);
-    if (top > 3.4e38f) {  // an infinity: once more, with NaN in its place
-      tops = 0;
+      fetch(plane_head + 4 * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      Piece<T> x[PASSES];
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
-        x[i].spoil();
-        tops = x[i].top(tops);
+        const int r = i * ROWS + row_in_pass;
+        if (row_in_pass < ROWS && r < n)
+          x[i].load(ring + stage * S::STAGE + i * PIECE);
+        else
+          x[i].clear();
       }
-      top = Piece<T>::top_of(tops);
-    }
-    const float s = fmaxf(s_old, scale_for(warp_max(top)));
-    const float inv = inverse_of(s);
-    if (continued && s > s_old) {
-      uint8_t* earlier = dst - (size_t)before * DH - col + (lane % LANES) * 8;
-      const float ratio = s_old * inv;
-      constexpr int TURN = PASSES < 4 ? PASSES : 4;  // under way at once: this is the longest way through a decode step
-#pragma unroll 1
-      for (int i0 = 0; i0 < PASSES; i0 += TURN) {
-        uint2 was[TURN];
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      const size_t page_head = (size_t)page * 2 * p.n_kv_heads + plane_head;
+      uint8_t* dst = p.pool + (page_head * p.page_size + row) * DH + col;  // of the first new token
+      float* scale_at = p.scales + page_head * (p.page_size / BLOCK) + row / BLOCK;
+      const float s_old = continued ? *scale_at : 0.f;
+      uint32_t tops = 0;
 #pragma unroll
-        for (int i = 0; i < TURN; ++i) {
-          const int r = (i0 + i) * ROWS + row_in_pass;
-          if (row_in_pass < ROWS && r < before) was[i] = *reinterpret_cast<const uint2*>(earlier + (size_t)r * DH);
+      for (int i = 0; i < PASSES; ++i) tops = x[i].top(tops);
+      float top = Piece<T>::top_of(tops);
+      if (top > 3.4e38f) {  // an infinity: once more, with NaN in its place
+        tops = 0;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          x[i].spoil();
+          tops = x[i].top(tops);
         }
+        top = Piece<T>::top_of(tops);
+      }
+      const float s = fmaxf(s_old, scale_for(warp_max(top)));
+      const float inv = inverse_of(s);
+      if (continued && s > s_old) {
+        uint8_t* earlier = dst - (size_t)before * DH - col + (lane % LANES) * 8;
+        const float ratio = s_old * inv;
+        constexpr int TURN = PASSES < 4 ? PASSES : 4;  // under way at once: this is the longest way through a decode step
+#pragma unroll 1
+        for (int i0 = 0; i0 < PASSES; i0 += TURN) {
+          uint2 was[TURN];
 #pragma unroll
-        for (int i = 0; i < TURN; ++i) {
-          const int r = (i0 + i) * ROWS + row_in_pass;
-          if (row_in_pass < ROWS && r < before) {
-            uint32_t out[2];
+          for (int i = 0; i < TURN; ++i) {
+            const int r = (i0 + i) * ROWS + row_in_pass;
+            if (row_in_pass < ROWS && r < before) was[i] = *reinterpret_cast<const uint2*>(earlier + (size_t)r * DH);
+          }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t u = h ? was[i].y : was[i].x;
-              const uint32_t lo = decode2((uint16_t)u), hi = decode2((uint16_t)(u >> 16));
-              const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              out[h] = (uint32_t)encode2(a.x * ratio, a.y * ratio) | ((uint32_t)encode2(b.x * ratio, b.y * ratio) << 16);
+          for (int i = 0; i < TURN; ++i) {
+            const int r = (i0 + i) * ROWS + row_in_pass;
+            if (row_in_pass < ROWS && r < before) {
+              uint32_t out[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t u = h ? was[i].y : was[i].x;
+                const uint32_t lo = decode2((uint16_t)u), hi = decode2((uint16_t)(u >> 16));
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                out[h] = (uint32_t)encode2(a.x * ratio, a.y * ratio) | ((uint32_t)encode2(b.x * ratio, b.y * ratio) << 16);
+              }
+              *reinterpret_cast<uint2*>(earlier + (size_t)r * DH) = make_uint2(out[0], out[1]);
             }
-            *reinterpret_cast<uint2*>(earlier + (size_t)r * DH) = make_uint2(out[0], out[1]);
           }
         }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = i * ROWS + row_in_pass;
-      if (row_in_pass < ROWS && r < n) {
-        x[i].template store<DH>(dst + (size_t)r * DH, inv);
+      for (int i = 0; i < PASSES; ++i) {
+        const int r = i * ROWS + row_in_pass;
+        if (row_in_pass < ROWS && r < n) x[i].template store<DH>(dst + (size_t)r * DH, inv);
       }
-    }
-    if (lane == 0) *scale_at = s;
+      if (lane == 0) *scale_at = s;
     }
   }
 }
