@@ -38,7 +38,7 @@ RL_EXPORT int rl_kv8_attention(int dtype, const void* q, long q_stride, const vo
   if (page_size <= 0 || page_size % rl::kv8::BLOCK != 0) return -4;
   if (row_blocks < 1 || sms < 0 || (rows != 8 && rows != 16 && rows != 32 && rows != 64 && rows != 128)) return -5;
   if (rows == 128 && (dtype != RL_BF16 || sms <= 0 || (head_dim != 64 && head_dim != 128) || page_size > 4096)) return -5;
-  if (n_kv_heads > 65535 || (long)n_items * row_blocks > 0x7fffffffL) return -6;
+  if (n_kv_heads > 65535 || (long)n_items * row_blocks > 0x7fffffffL / (sms == 0 ? n_kv_heads : 1)) return -6;
   if (sms > 0 && (blocks < 1 || plan == nullptr || part_o == nullptr || part_ml == nullptr)) return -7;
   if (status == nullptr) return -8;
   const rl::kv8::AttnParams8 p{q,     q_stride, (const uint8_t*)pool, scales,     block_table, bt_rows,    bt_cols,   q_start, kv_len,

@@ -281,12 +281,12 @@ __device__ __forceinline__ void multiply_keys(
 }
 
 // The softmax's step over the scores of a tile, and O^T += V^T P^T.  ks, vs: the blocks' scales; ks negative: a block that is not there.
-// v_of(b, v): the lane's words of the values of block b, rows c, c + 4, c + 8, c + 12.  SIGHT: every row sees every key (WHOLE), all rows see the same
+// v_of(b, v): the lane's words of the values of block b, rows c, c + 4, c + 8, c + 12.  sight: every row sees every key (WHOLE), all rows see the same
 // (ALIKE: decoded tokens), or not; key0 is the first key's position and pos the lane's rows'.  A tile is nearly always whole, and the checks
-// are as many instructions as the rest.
+// are as many instructions as the rest.  (One body with branches that all lanes take alike: three bodies, one a sight, were no faster.)
 enum Sight { WHOLE, ALIKE, APART };
-template <int DH, bool F32, int NR, Sight SIGHT, class VOf>
-__device__ __forceinline__ void use_scores(State<DH, NR>& st, float (&s)[Shapes<DH, F32, NR>::TB][NR][4], VOf v_of,
+template <int DH, bool F32, int NR, class VOf>
+__device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st, float (&s)[Shapes<DH, F32, NR>::TB][NR][4], VOf v_of,
                                            const float (&ks)[Shapes<DH, F32, NR>::TB], const float (&vs)[Shapes<DH, F32, NR>::TB],
                                            const float (&factor)[NR][2], int key0, const int (&pos)[NR][2], int window) {
   using S = Shapes<DH, F32, NR>;
@@ -298,12 +298,16 @@ __device__ __forceinline__ void use_scores(State<DH, NR>& st, float (&s)[Shapes<
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[n][i] = NOTHING;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int b = 0; b < TB; ++b) {
-        f[b][n][i] = factor[n][i] * ks[b];
-        if constexpr (SIGHT != WHOLE) {
+      for (int b = 0; b < TB; ++b) f[b][n][i] = factor[n][i] * ks[b];
+  if (sight != WHOLE) {
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int key = key0 + b * BLOCK + key_row + 8 * h;
@@ -312,8 +316,14 @@ __device__ __forceinline__ void use_scores(State<DH, NR>& st, float (&s)[Shapes<
           }
           f[b][n][i] = 1.f;
         }
-        top[n][i] = fmaxf(top[n][i], fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i]);
-      }
+  }
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[n][i] = NOTHING;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) top[n][i] = fmaxf(top[n][i], fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i]);
     }
   bool grown = false;
 #pragma unroll
@@ -376,7 +386,7 @@ __device__ __forceinline__ void use_scores(State<DH, NR>& st, float (&s)[Shapes<
     v_of(b, v);
     // Where a row does not see every key, a value that is NaN (of a token it does not see, or of whatever lies behind the last key) must not
     // reach it: 0 * NaN is NaN.  Such codes are counted row by row over the keys that the row does see, and taken out of the product.
-    if constexpr (SIGHT == ALIKE) {  // (no row sees a key that its neighbour does not: the hidden keys' values are no value at all)
+    if (sight == ALIKE) {  // (no row sees a key that its neighbour does not: the hidden keys' values are no value at all)
       const int c = lane & 3;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -386,7 +396,7 @@ __device__ __forceinline__ void use_scores(State<DH, NR>& st, float (&s)[Shapes<
         for (int t = 0; t < DH / 32; ++t) v[i][t] = hidden ? 0u : v[i][t];
       }
     }
-    if constexpr (SIGHT == APART) {
+    if (sight == APART) {
       bool nan = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -492,8 +502,8 @@ __device__ __forceinline__ void ask_for_block(uint32_t answer, uint32_t bar) {
   tc::mbar_expect_tx(bar, 16);
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
 }
-__device__ __forceinline__ bool read_answer(uint32_t answer, int& x, int& y) {
-  uint32_t there;
+__device__ __forceinline__ bool read_answer(uint32_t answer, int& x) {
+  uint32_t there, y;
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t"
       "ld.shared.b128 h, [%3];\n\t"
@@ -516,7 +526,9 @@ __device__ __forceinline__ bool read_answer(uint32_t answer, int& x, int& y) {
 // 1: the tiles of all units in a row, and in front of each unit's the cost of beginning one, are cut into as many equal runs as blocks stand on the device
 // at once (but runs of at least p.cost + 4 tiles, or of up to p.cost + 16 where there is one for each SM), whatever the lengths.  A unit that a
 // run has the whole of goes to the output; of others, a run has at most two, and kv8_join_kernel joins their parts.  32 contexts of up to 16384 tokens, 8 heads of 128: 114 us in parts of 1536
-// keys that blocks take over from one another, which leaves the last of them waiting for the longest.
+// keys that blocks take over from one another, which leaves the last of them waiting for the longest; 102 so, of 85 of traffic.
+// What bounds it where units are short (64 decoded tokens of 25 heads of 64 and up to 1023 keys: 39 us, 16.6 of traffic) is latency: a block takes
+// 17,000 cycles for a unit of ten tiles, of which its warps compute 6,600; fifteen warps an SM issue in 29 % of the cycles.
 //
 // The fetching warp tells the others what comes next by a segment, two of which may be open, and lays the queries out for them (decoded tokens: the
 // loads of queries, and all that hangs on the batch's description, are then as far ahead as the keys).  Codes and scales come by
@@ -670,23 +682,24 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
     };
 
     if (p.balanced) {
-      const int total = before[p.n_entries] * p.n_kv_heads, blocks = (int)gridDim.x;
-      const int run = max((total + blocks - 1) / blocks, min(max((total + p.balanced - 1) / p.balanced, p.cost + 4), p.cost + 16));
+      const long total = (long)before[p.n_entries] * p.n_kv_heads;  // (more than 2^31 for thousands of rows' blocks over a million tokens)
+      const int blocks = (int)gridDim.x;
+      const int run = (int)max((total + blocks - 1) / blocks, min(max((total + p.balanced - 1) / p.balanced, p.cost + 4L), p.cost + 16L));
       if (blockIdx.x == 0) {  // for the kernel that joins
         for (int e = lane; e <= p.n_entries; e += 32) p.plan[1 + e] = before[e];
         if (lane == 0) p.plan[0] = run;
       }
-      int at = blockIdx.x * run;
-      const int end = min(total, at + run);
+      long at = (long)blockIdx.x * run;
+      const long end = min(total, at + run);
       int entry = 0;  // the last entry that begins at or before `at`
       for (int hi = p.n_entries; hi - entry > 1;) {
         const int mid = (entry + hi) >> 1;
-        if (before[mid] * p.n_kv_heads <= at)
+        if ((long)before[mid] * p.n_kv_heads <= at)
           entry = mid;
         else
           hi = mid;
       }
-      int rest = at - before[entry] * p.n_kv_heads;  // of the entry, that earlier runs have
+      int rest = (int)(at - (long)before[entry] * p.n_kv_heads);  // of the entry, that earlier runs have
       __syncwarp();  // the last reading of `before`; the other warps are past it too (the ring is written from here on)
       for (; at < end && ok; ++entry) {
         const Work w = work_of<L::RB>(p, entry);
@@ -695,26 +708,27 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
         int h = rest / (p.cost + tiles), off = rest - h * (p.cost + tiles);
         rest = 0;
         for (; h < p.n_kv_heads && at < end && ok; ++h) {
-          const int n = min(p.cost + tiles - off, end - at), i0 = max(off - p.cost, 0), i1 = max(off + n - p.cost, 0);
+          const int n = (int)min((long)(p.cost + tiles - off), end - at), i0 = max(off - p.cost, 0), i1 = max(off + n - p.cost, 0);
           if (i1 > i0) serve(w, h, i0, i1, i1 - i0 == tiles ? -1 : (int)blockIdx.x * 2 + (off >= p.cost ? 0 : 1));
           at += n;
           off = 0;
         }
       }
     } else {
-      int x = blockIdx.x, y = blockIdx.y;
+      int unit = blockIdx.x;  // heads of an entry next to one another: their blocks of a page lie so too, and are read at about the same time
       for (uint32_t n = 0;; ++n) {
         if (lane == 0) ask_for_block(base + L::ANSWER, base + L::ASK);
         __syncwarp();
-        const Work w = work_of<L::RB>(p, x);
+        const int entry = unit / p.n_kv_heads;
+        const Work w = work_of<L::RB>(p, entry);
         const int tiles = w.tiles(TB);
-        if (tiles > 0 && ok) serve(w, y, 0, tiles, -1);
+        if (tiles > 0 && ok) serve(w, unit - entry * p.n_kv_heads, 0, tiles, -1);
         // the answer is waited for whatever happens: it is on its way into this block's shared memory
         if (!tc::mbar_wait_warp(base + L::ASK, n & 1u, abort_flag, p.status)) {
           if (lane == 0) tc::mbar_wait_quiet(base + L::ASK, n & 1u);
           ok = false;
         }
-        if (!ok || !read_answer(base + L::ANSWER, x, y)) break;
+        if (!ok || !read_answer(base + L::ANSWER, unit)) break;
       }
     }
     if (ok) {
@@ -807,12 +821,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
 #pragma unroll
           for (int j = 0; j < 4; ++j) load_words<DH / 32>(codes + L::PLANE + (b * BLOCK + c + 4 * j) * DH + r * (DH / 8), v[j]);
         };
-        if (whole)
-          use_scores<DH, F32, NR, WHOLE>(st, s, v_of, ks, vs, factor, key0, pos, p.window);
-        else if (pos_lo == pos_hi)
-          use_scores<DH, F32, NR, ALIKE>(st, s, v_of, ks, vs, factor, key0, pos, p.window);
-        else
-          use_scores<DH, F32, NR, APART>(st, s, v_of, ks, vs, factor, key0, pos, p.window);
+        use_scores<DH, F32, NR>(whole ? WHOLE : pos_lo == pos_hi ? ALIKE : APART, st, s, v_of, ks, vs, factor, key0, pos, p.window);
       }
       __syncwarp();
       if (lane == 0) arrive(base + L::EMPTY + 8 * slot);
@@ -916,7 +925,8 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   pdl_begin();
   const int run = p.plan[0], mine = p.plan[1 + blockIdx.x], cost = p.plan[2 + blockIdx.x] - mine;
   if (cost <= 0) return;
-  const int begin = mine * p.n_kv_heads + blockIdx.y * cost + p.cost, first = begin / run, parts = (begin + cost - p.cost - 1) / run - first + 1;
+  const long begin = (long)mine * p.n_kv_heads + (long)blockIdx.y * cost + p.cost;
+  const int first = (int)(begin / run), parts = (int)((begin + cost - p.cost - 1) / run) - first + 1;
   if (parts <= 1) return;
   const Work w = work_of<RB>(p, blockIdx.x);
   const Rows rows{w.token0, w.pos0, w.first_row, w.rows, (int)blockIdx.y};
@@ -984,7 +994,7 @@ int launch_attention(AttnParams8 p, int most_rows, int blocks, Fit* fit, cudaStr
   const auto kernel = kv8_attention_kernel<DH, F32, NR, WR>;
   const int rc = (int)note_launch(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f.bytes));
   if (rc != 0) return take_launch_error();
-  launch_pdl_all_shared(kernel, p.balanced ? dim3(blocks) : dim3(p.n_entries, p.n_kv_heads), dim3(160), f.bytes, stream, p);
+  launch_pdl_all_shared(kernel, p.balanced ? dim3(blocks) : dim3((unsigned)p.n_entries * p.n_kv_heads), dim3(160), f.bytes, stream, p);
   if (p.balanced) launch_pdl(kv8_join_kernel<F32, L::RB>, dim3(p.n_entries, p.n_kv_heads, L::RB / 8), dim3(128), 0, stream, p);
   return 0;
 }
