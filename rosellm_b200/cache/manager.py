@@ -249,6 +249,12 @@ class CacheManager:
         whole, rest = divmod(cur, self.page_size)
         if self.slots.num_free < 1 or (rest and any(g.allocator.num_free < 1 for g in self.groups)):
             return None
+        if self.device.type == "cuda":
+            from ..ops.kernels import PagePools
+
+            for g in self.groups:  # before anything is taken: it refuses pools that cannot be copied
+                if g.page_pools is None and g.pools:
+                    g.page_pools = PagePools([*g.pools.values(), *g.scales.values()])
         new = self.slots.alloc(1)[0]
         self.num_tokens[new] = cur
         for g in self.groups:
@@ -276,11 +282,10 @@ class CacheManager:
             for t in (*g.pools.values(), *g.scales.values()):
                 t[dst].copy_(t[src])
             return
-        from ..ops.kernels import PagePools, copy_pages
+        from ..ops.kernels import copy_pages
 
-        if g.page_pools is None:
-            g.page_pools = PagePools([*g.pools.values(), *g.scales.values()])
-        copy_pages(g.page_pools, torch.tensor([[src, dst]], dtype=torch.int32, device=self.device))
+        with torch.cuda.device(self.device):
+            copy_pages(g.page_pools, torch.tensor([[src, dst]], dtype=torch.int32, device=self.device))
 
     def release(self, slot: int) -> None:
         """The request is over (finished, aborted or preempted): everything it holds goes back."""

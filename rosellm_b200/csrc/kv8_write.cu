@@ -282,7 +282,7 @@ int launch_write(const WriteParams& p, int dh, cudaStream_t stream) {
   // prompt portions one token in 16 leads, and a block of threads looks at 16 tokens, or 4 where the step is mixed.
   const int group = (long)p.n_tokens >= 32L * p.n_reqs ? 16 : (long)p.n_tokens >= 4L * p.n_reqs ? 4 : 1;
   // Planes a warp: more share the looking up and the beginning of a block, as long as one or two rounds of blocks are left for the device's 148 SMs.
-  // Measured, us with 1 / 2 / 4: 24 portions of 512, 16 heads of 64 (6144 blocks of one) 26.5 / 19.0 / 16.6, 8 of 128 (3072) 18.9 / 16.8 / 18.5; decode steps
+  // Measured, us with 1 / 2 / 4: 24 portions of 512, 16 heads of 64 (6144 blocks of one) 26.5 / 19.0 / 16.6, 8 of 128 (half as many) 18.9 / 16.8 / 18.5; decode steps
   // of 256, 16 of 64 (2048) 7.7 / 6.5 / 7.0, 8 of 128 in 32 bits (1024) 5.8 / 7.0 / 6.2, of 64, 16 of 64 (512) 3.4 / 3.7 / 4.4.
   const long tokens = (p.n_tokens + group - 1) / group;
   auto blocks_of = [&](int each) { return tokens * ((2 * p.n_kv_heads + 4 * each - 1) / (4 * each)); };
