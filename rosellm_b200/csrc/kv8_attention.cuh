@@ -109,6 +109,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// d += a (hi + lo), hi and lo the halves of a 32-bit operand.  The instruction cuts its sums off, always towards zero, which adds up over a head of 256
+// or a context of thousands; so its sums are of one step of 16 alone, and those are added by rounding.  Measured (relative to 64 bits, heads of
+// 256, 2000 keys): 4.4e-7, in one sum 1.6e-6, summed plainly in 32 bits 1.3e-6.
+__device__ __forceinline__ void add_both(float (&d)[4], const uint32_t (&a)[4], uint32_t hi0, uint32_t hi1, uint32_t lo0, uint32_t lo1) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  mma16816(x, a, lo0, lo1);
+  mma16816(x, a, hi0, hi1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] += x[i];
+}
+
 // An 8 x 8 matrix of halves, a row of it in four lanes, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
@@ -273,9 +284,12 @@ __device__ __forceinline__ void multiply_keys(
       const uint32_t a[4] = {decode2((uint16_t)kw[b][0][k]), decode2((uint16_t)kw[b][1][k]), decode2((uint16_t)(kw[b][0][k] >> 16)),
                              decode2((uint16_t)(kw[b][1][k] >> 16))};
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int qp = 0; qp < S::QPARTS; ++qp) mma16816(s[b][n], a, q[n][qp].x, q[n][qp].y);
+      for (int n = 0; n < NR; ++n) {
+        if constexpr (F32)
+          add_both(s[b][n], a, q[n][0].x, q[n][0].y, q[n][1].x, q[n][1].y);
+        else
+          mma16816(s[b][n], a, q[n][0].x, q[n][0].y);
+      }
     }
   }
 }
@@ -442,8 +456,10 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
         const uint32_t a[4] = {decode2((uint16_t)x), decode2((uint16_t)(x >> 16)), decode2((uint16_t)y), decode2((uint16_t)(y >> 16))};
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          mma16816(st.o[n][2 * t + h], a, hi[n][0], hi[n][1]);
-          if constexpr (F32) mma16816(st.o[n][2 * t + h], a, lo[n][0], lo[n][1]);
+          if constexpr (F32)
+            add_both(st.o[n][2 * t + h], a, hi[n][0], hi[n][1], lo[n][0], lo[n][1]);
+          else
+            mma16816(st.o[n][2 * t + h], a, hi[n][0], hi[n][1]);
         }
       }
   }
