@@ -201,3 +201,42 @@ def test_models_that_8_bits_do_not_fit(tmp_path):
         InferenceEngine(tiny_lebedra.write_tiny(name, str(tmp_path)), kv_cache_dtype="fp8")
     with pytest.raises(ConfigError, match="multiple of 16"):
         engine(write_tiny("B", str(tmp_path)), page_size=8)
+
+
+@pytest.mark.parametrize("family,name", [("", "B_sharp"), ("lebedra", "X"), ("porovik", "A"), ("porovik", "B"), ("fikevik", "A"), ("fikevik", "B"), ("soporax", "A"),
+                                         ("soporax", "B"), ("vebotar", "A"), ("vebotar", "B"), ("kugadra", "A"), ("kugadra", "B")])
+def test_forks_of_other_caches(family, name, tmp_path):
+    """Latent rows, biased rows, windows, chunks, states and several copies of a stack, in the engine's own type: a fork and the first request, going on
+    with the same tokens and with others, each give what a request gives that was never forked.  Both sides lie within 1e-4 of the logits' size
+    of the formulas (the replay tests' tolerance of 32 bits), so within twice that of one another."""
+    import importlib
+    import inspect
+
+    from rosellm_b200.engine.llm import InferenceEngine
+
+    mod = importlib.import_module(f"tiny_{family}" if family else "tiny")
+    more = dict(decisive=True) if "decisive" in inspect.signature(mod.write_tiny).parameters else {}
+    r = InferenceEngine(mod.write_tiny(name, str(tmp_path), **more), dtype="float32", page_size=mod.TINY[name]["page_size"], max_batch_size=6,
+                        kv_cache_max_tokens=1024, cuda_graphs=False).runner
+    vocab = r.config.vocab_size if hasattr(r.config, "vocab_size") else 100
+    rng = np.random.default_rng(5)
+    prompt = rng.integers(0, vocab, 37).tolist()
+    steps = [([t], [t]) for t in rng.integers(0, vocab, 2).tolist()] + [(rng.integers(0, vocab, 5).tolist(), rng.integers(0, vocab, 5).tolist()), ([3], [4]), ([6], [6])]
+    a = r.cache.new_request()
+    r.step([entry(a, prompt[:20], [])])
+    r.step([entry(a, prompt[20:], [])])
+    b = r.fork(a)
+    r.cache.check()
+    got = [r.step([entry(a, x, list(range(len(x)))), entry(b, y, list(range(len(y))))]).clone() for x, y in steps]
+    r.cache.check()
+    r.cache.release(a)
+    r.cache.release(b)
+    r.cache.check()
+    alone = [r.cache.new_request() for _ in range(2)]
+    for s in alone:
+        r.step([entry(s, prompt[:20], [])])
+        r.step([entry(s, prompt[20:], [])])
+    for g, (x, y) in zip(got, steps):
+        want = r.step([entry(alone[0], x, list(range(len(x)))), entry(alone[1], y, list(range(len(y))))])
+        torch.testing.assert_close(g, want, rtol=0, atol=2e-4 * max(1.0, float(want.abs().max())))
+    r.check_status()

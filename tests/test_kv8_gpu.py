@@ -459,3 +459,33 @@ def test_refusals(K):
     with pytest.raises(K.KernelError, match=r"\[n, 2\]"):
         K.copy_pages(K.PagePools([pool]), torch.zeros(3, dtype=torch.int32, device=DEV))
     K.check_status(DEV)
+
+
+# ---- calls beside one another, pages of other sizes ------------------------------------------------
+
+@pytest.mark.parametrize("page", [1024, 4096, 8192])
+def test_large_pages(K, page):
+    """Few large pages, of more tokens than the tcgen05 kernel's division takes as well; decoded tokens beside portions of 64 rows and more."""
+    check_attention(K, [(700, 64), (1030, 1), (600, 20), (5, 1)], 4, 1, 64, page, BF16)
+
+
+def test_two_streams(K):
+    """Two calls that may run at the same time, each with scratch of its own and none, on streams that are not the default one."""
+    gen = torch.Generator().manual_seed(9)
+    jobs = []
+    for each in ([(3000, 1)] * 3, [(2500, 40), (900, 64)]):
+        batch = P.Batch(each, 16, seed=len(each))
+        pool, scales = cache_of(batch, 2, 128, gen)
+        q = torch.randn(batch.tokens, 1024, generator=gen).to(BF16)
+        want = P.attention(batch, q.double().unflatten(1, (8, 128)), P.values_of(pool), scales.double(), 8, 128 ** -0.5)
+        jobs.append((batch, pool.to(DEV), scales.to(DEV), q.to(DEV), want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for turn in range(4):
+        for batch, pool, scales, q, want, stream in jobs:
+            with torch.cuda.stream(stream):
+                outs.append((do_attention(K, batch, q, pool, scales, 8), want))
+    torch.cuda.synchronize()
+    for out, (o, rough, fine) in outs:
+        compare(out, o, rough, fine, BF16)
+    K.check_status(DEV)
