@@ -240,3 +240,14 @@ def test_forks_of_other_caches(family, name, tmp_path):
         want = r.step([entry(alone[0], x, list(range(len(x)))), entry(alone[1], y, list(range(len(y))))])
         torch.testing.assert_close(g, want, rtol=0, atol=2e-4 * max(1.0, float(want.abs().max())))
     r.check_status()
+
+
+def test_the_command_line(folder):
+    """The ids that the command line prints with ``--kv-cache-dtype fp8`` are those that the engine gives with the same options."""
+    from test_cli_gpu import printed_ids, run_cli
+
+    prompt = [5, 17, 3, 250, 9, 44, 101]
+    out = run_cli("--model", folder, "--dtype", "fp32", "--kv-cache-dtype", "fp8", "--prompt-ids", ",".join(map(str, prompt)), "--max-new-tokens", "8",
+                  "--no-stop-on-eos")
+    e = engine(folder)
+    assert printed_ids(out, False) == e.generate_batch([prompt], max_new_tokens=8, stop_on_eos=False)[0]
