@@ -3,6 +3,7 @@
 // A copy moves each byte twice, so its floor is the memory's copy bandwidth; what costs otherwise is one launch a pool (two a layer).
 // A block of threads takes a run of 16-byte units (4-byte ones where a page's size is no multiple of 16) of one pool's
 // copies, several loads of a thread on their way before its first store.
+// Measured: 1024 pages of 24 layers 245 us, the copy bandwidth (a pool at a time with indexing 7,588); one page of 12 layers 3.0 us, a launch.
 #include "common.cuh"
 
 namespace rl {
