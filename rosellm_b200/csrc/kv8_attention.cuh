@@ -733,6 +733,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
     } else {
       int unit = blockIdx.x;  // heads of an entry next to one another: their blocks of a page lie so too, and are read at about the same time
       for (uint32_t n = 0;; ++n) {
+        __syncwarp();  // the answer before this one has been read by every lane: the next goes into the same place
         if (lane == 0) ask_for_block(base + L::ANSWER, base + L::ASK);
         __syncwarp();
         const int entry = unit / p.n_kv_heads;
