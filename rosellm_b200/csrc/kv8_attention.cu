@@ -41,6 +41,7 @@ RL_EXPORT int rl_kv8_attention(int dtype, const void* q, long q_stride, const vo
   if (n_kv_heads > 65535 || (long)n_items * row_blocks > 0x7fffffffL / (sms == 0 ? n_kv_heads : 1)) return -6;
   if (sms > 0 && (blocks < 1 || plan == nullptr || part_o == nullptr || part_ml == nullptr)) return -7;
   if (status == nullptr) return -8;
+  if (n_pages < 1) return -11;  // (the tcgen05 kernel reads the first page in the place of one that is not there)
   const rl::kv8::AttnParams8 p{q,     q_stride, (const uint8_t*)pool, scales,     block_table, bt_rows,    bt_cols,   q_start, kv_len,
                                slots, out,      out_stride,           items,      is_tiles,    n_tokens,   n_heads,   n_kv_heads, head_dim,
                                page_size, n_pages, window,            scale,      row_blocks,  n_items * row_blocks, sms, 0, plan,

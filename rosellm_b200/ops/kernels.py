@@ -2280,6 +2280,8 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     at the same time need scratch of their own."""
     global _launches
     here, pool_at, n_pages, n_kv, page_size, dh = _kv8_pool(pool, scales, "kv8_attention")
+    if n_pages == 0:
+        raise KernelError("kv8_attention: the pool has no page")
     if n_heads <= 0 or n_heads % n_kv != 0:
         raise KernelError(f"kv8_attention: {n_heads} heads are not a multiple of {n_kv} key/value heads")
     code, n_tokens, q_stride, q_at, out_rows, out_stride, out_at = _kv8_rows("kv8_attention", ("q", "out"), q, out, n_heads * dh, here)
@@ -2288,7 +2290,7 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     _kv8_ints(here, "block_table q_start kv_len slots", block_table, q_start, kv_len, slots)
     table = block_table.shape
     n_reqs = q_start.numel() - 1
-    if len(table) != 2 or kv_len.numel() < n_reqs or slots.numel() < n_reqs:
+    if len(table) != 2 or n_reqs < 0 or kv_len.numel() < n_reqs or slots.numel() < n_reqs:
         raise KernelError("kv8_attention: block_table must be [slots, pages], q_start one longer than there are requests, kv_len and slots as long")
     if n_tiles > 0:
         if tiles is None:
@@ -2302,6 +2304,8 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
         _kv8_ints(here, "decode_reqs", decode_reqs)
         if decode_reqs.numel() < n_decode:
             raise KernelError("kv8_attention: decode_reqs is shorter than n_decode")
+    if n_reqs == 0 and (n_tiles > 0 or n_decode > 0):
+        raise KernelError("kv8_attention: tiles or decoded requests of a batch without requests")
     if window is not None and window <= 0:
         raise KernelError("kv8_attention: a window sees at least one key")
     if n_tokens == 0:

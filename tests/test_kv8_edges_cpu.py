@@ -2,6 +2,10 @@
 import os
 import re
 
+import torch
+
+from rosellm_b200.ops import kernels as K
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rosellm_b200", "csrc")
 
 
@@ -13,3 +17,14 @@ def test_the_next_block_is_asked_for_when_all_lanes_have_read_the_answer():
     asking = [body for body in loops if "ask_for_block(" in body]
     assert len(asking) == 1 == len(re.findall(r"\bask_for_block\(base", source)) == len(re.findall(r"\bread_answer\(base", source))
     assert "__syncwarp();" in asking[0].split("ask_for_block(")[0]
+
+
+def test_a_pool_without_pages_is_refused():
+    """The tcgen05 kernel reads the pool's first page in the place of one that is not there (its keys are hidden): there has to be one."""
+    at = torch.zeros(64).data_ptr()
+
+    def attend(rows, sms, n_pages):
+        return K._lib().rl_kv8_attention(1, at, 128, at, at, at, 1, 1, at, at, at, at, 128, at, 1, 1, 1, 2, 1, 64, 16, n_pages, 0, 1.0,
+                                         rows, 1, sms, 148, at, at, at, at, None)
+
+    assert [attend(128, 148, 0), attend(8, 0, 0), attend(64, 148, -1)] == [-11] * 3
