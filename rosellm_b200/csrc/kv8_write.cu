@@ -101,7 +101,7 @@ struct Piece<float> {
     for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(get(i)));
     return __float_as_uint(t);
   }
-  static __device__ __forceinline__ float spoilt(float f) { return fabsf(f) <= 3.4e38f ? f : CUDART_NAN_F; }
+  static __device__ __forceinline__ float spoilt(float f) { return fabsf(f) < CUDART_INF_F ? f : CUDART_NAN_F; }
   __device__ __forceinline__ void spoil() {
     a = make_float4(spoilt(a.x), spoilt(a.y), spoilt(a.z), spoilt(a.w));
     b = make_float4(spoilt(b.x), spoilt(b.y), spoilt(b.z), spoilt(b.w));
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(128, WriteShape<T, DH>::AT_ONCE) void kv8_write_ker
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) tops = x[i].top(tops);
       float top = Piece<T>::top_of(tops);
-      if (top > 3.4e38f) {  // an infinity: once more, with NaN in its place
+      if (top == CUDART_INF_F) {  // an infinity: once more, with NaN in its place
         tops = 0;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {

@@ -28,3 +28,19 @@ def test_batches_without_a_request_or_a_page_are_refused(K):
             attend(**change)
     attend(q_start=ints(0), n_tiles=0)  # nothing to do is no fault
     K.check_status(DEV)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_largest_finite_values_are_values(K, dtype):
+    """Entries from 3.4e38 to the largest finite one of the type are stored and count for the scale, also beside infinities; rows that are continued too."""
+    most = torch.finfo(dtype).max
+    batch = P.Batch([(40, 40), (25, 5), (20, 4)], 16)
+    gen = torch.Generator().manual_seed(11)
+    pool, scales = T.cache_of(batch, 1, 64, gen)
+    k, v = (torch.randn(batch.tokens, 64, generator=gen).to(dtype) for _ in range(2))
+    k[0, 0], k[3, 9], k[20, 63] = most, -most, most
+    k[16:32, 5] = torch.tensor(3.401e38, dtype=torch.float64).to(dtype) if dtype == F32 else most
+    v[33, 1], v[34, 2], v[35, 3] = most, float("inf"), float("nan")  # the largest beside what is none
+    k[41, 7], v[46, 8] = -most, most  # in blocks that hold earlier tokens
+    dp, _ = T.check_write(K, batch, 1, 64, dtype, k, v, pool, scales)
+    assert int(torch.isnan(dp.float()).sum()) == 2
