@@ -222,8 +222,8 @@ struct Queries {
 #pragma unroll
       for (int k = 0; k < DH / 32; ++k) top = fmaxf(top, fabsf(x[n][k]));
       top = warp_max(top);
-      // the power of two that puts the largest entry between 2^14 and 2^15 (kept within the exponents whose inverse is a float)
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 126);
+      // the power of two that puts the largest entry between 2^14 and 2^15 (kept within the exponents for which both factors are normal numbers)
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 127);
       const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23), down = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
       if (lane == 0) factor[r] = down * p.scale * 1.4426950408889634f;
 #pragma unroll

@@ -380,7 +380,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = max3(top, fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xFFFF0000u)));
         }
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 126);
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 127);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
         factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
 #pragma unroll

@@ -44,3 +44,23 @@ def test_the_largest_finite_values_are_values(K, dtype):
     k[41, 7], v[46, 8] = -most, most  # in blocks that hold earlier tokens
     dp, _ = T.check_write(K, batch, 1, 64, dtype, k, v, pool, scales)
     assert int(torch.isnan(dp.float()).sum()) == 2
+
+
+def on_tcgen05(K, each, heads, n_kv, dim, page, window=None):
+    """Whether the portions of such a batch run on the tcgen05 kernel."""
+    plan = K.kv8_attention_plan(dtype=BF16, n_heads=heads, n_kv=n_kv, head_dim=dim, page_size=page, span=max(n for n, _ in each), window=window,
+                                n_tiles=sum(-(-k // 64) for _, k in each if k > 1), max_q=max(k for _, k in each))[0]
+    return plan is not None and plan[0] == 128
+
+
+@pytest.mark.parametrize("dtype,each", [(F32, [(200, 1), (150, 40)]), (BF16, [(200, 1), (150, 20)]), (BF16, [(600, 70), (40, 1)])])
+def test_queries_of_the_largest_size(K, dtype, each):
+    """Queries up to the largest finite value over keys of the smallest scale: their scores are ordinary numbers."""
+    def touch(batch, q, pool, scales):
+        top = q.float().abs().unflatten(1, (2, 64)).amax(dim=2, keepdim=True)
+        q.copy_((q.float().unflatten(1, (2, 64)) / top * torch.finfo(dtype).max).flatten(1).to(dtype))
+        assert torch.isfinite(q).all() and (q.abs() > 2.0 ** 127).any(dim=1).all()
+        scales[:, 0] = 2.0 ** -126
+
+    T.check_attention(K, each, 2, 2, 64, 16, dtype, touch=touch)
+    assert on_tcgen05(K, each, 2, 2, 64, 16) == (each[0][1] == 70)
