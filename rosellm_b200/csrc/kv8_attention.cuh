@@ -14,9 +14,13 @@
 // and 2c+1 are keys c and c+4, so that neighbouring lanes read neighbouring rows of V.  P^T is S^T's fragment transposed in registers (movmatrix).
 //
 // Scales: the 16 keys of a block share a key scale, by which their scores are multiplied.  A block of values is one inner step of P V, so its
-// probabilities are multiplied by (scale / largest scale so far) * 2^15 before they are rounded to halves (probabilities down to 2^-29 keep
-// all of their 11 bits: relative error 2^-11, against 2^-8 of a bfloat16 output), and the output follows the largest scale as it follows the
-// maximum.  Q is brought to halves row by row with a power of two that puts its largest entry at 2^14 (a bfloat16 fits exactly,
+// probabilities are multiplied by its scale.  The outputs therefore have a maximum of their own beside the softmax's: T, the largest score + log2(value
+// scale) that the row has seen, rounded up; probabilities enter P V as halves of 2^(score + log2 scale - T + 15).  The key that moves the output most thus
+// stands between 2^14 and 2^15 whatever the scales are, keys down to 2^-29 of it keep all of their 11 bits (relative error 2^-11, against 2^-8 of a
+// bfloat16 output), and none is off by more than 2^-40 of it.  What a row does not see has no part in T.  (Probabilities against the largest scale so
+// far, which may belong to keys of no weight or out of sight, lost bits from a ratio of 2^-18 on and everything at 2^-40.)  The
+// sum of the probabilities needs no row's maximum: each lane has its own for its own keys.  Both maxima are whole numbers, so that all changes of them are exact.
+// Q is brought to halves row by row with a power of two that puts its largest entry at 2^14 (a bfloat16 fits exactly,
 // within 2^-28 of the row's largest); in 32 bits Q and P are two halves each, a value and what its rounding left, so that products
 // are exact to 2^-22.  Sums, maxima and outputs are float32.
 #pragma once
@@ -100,6 +104,13 @@ struct Rows {
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The same with results down to 2^-149.
+__device__ __forceinline__ float ex2_small(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -245,19 +256,17 @@ constexpr float NOTHING = -1.7e38f;  // the maximum of no score: finite, so that
 template <int DH, int NR>
 struct State {
   float o[NR][DH / 16][4];  // tile i: entries [0], [1] are dim r * DH / 8 + 2 i of the two rows (r = lane / 4), [2], [3] the dim after it
-  float m[NR][2], l[NR][2]; // maximum (in units of log 2) and sum; the sum is over this lane's keys only until the end
-  float ref, inv;           // o is the sum of p * v / ref * 2^15; ref: the largest value scale so far, inv: 1 / ref (both 0 at first)
+  float t[NR][2];           // the rows' largest score + log2(value scale), in units of log 2, rounded up; o is the sum of 2^(score - t + 15) * v
+  float m[NR][2], l[NR][2]; // the largest score of this lane's keys, rounded up, and the sum of 2^(score - m + 15) over them
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) m[n][i] = NOTHING, l[n][i] = 0.f;
+      for (int i = 0; i < 2; ++i) t[n][i] = m[n][i] = NOTHING, l[n][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < DH / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
-    ref = inv = 0.f;
   }
-  __device__ __forceinline__ float unit() const { return ref * 3.0517578125e-05f; }  // what brings o to its own scale: ref * 2^-15
 };
 
 // S^T = K Q^T of TB blocks of 16 keys: kw[b][half] are the lane's words of its two keys of block b.
@@ -331,22 +340,28 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
           f[b][n][i] = 1.f;
         }
   }
+  float lv[TB];  // log2 of the value scales
 #pragma unroll
-  for (int n = 0; n < NR; ++n)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[n][i] = NOTHING;
-#pragma unroll
-      for (int b = 0; b < TB; ++b) top[n][i] = fmaxf(top[n][i], fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i]);
-    }
+  for (int b = 0; b < TB; ++b) lv[b] = (float)((int)(__float_as_uint(vs[b]) >> 23) - 127);
   bool grown = false;
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      float own = NOTHING;
+      top[n][i] = NOTHING;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) {
+        const float y = fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i];
+        own = fmaxf(own, y);
+        top[n][i] = fmaxf(top[n][i], y + lv[b]);
+      }
+      const float m = fmaxf(st.m[n][i], ceilf(own));
+      st.l[n][i] *= ex2(st.m[n][i] - m);
+      st.m[n][i] = m;
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], o));
-      grown |= top[n][i] > st.m[n][i];
+      grown |= top[n][i] > st.t[n][i];
     }
   if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -354,10 +369,9 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
       float turn[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float m = fmaxf(st.m[n][i], top[n][i]);
-        turn[i] = ex2(st.m[n][i] - m);
-        st.m[n][i] = m;
-        st.l[n][i] *= turn[i];
+        const float t = fmaxf(st.t[n][i], ceilf(top[n][i]));
+        turn[i] = ex2(st.t[n][i] - t);
+        st.t[n][i] = t;
       }
 #pragma unroll
       for (int t = 0; t < S::MT; ++t) {
@@ -366,20 +380,15 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
       }
     }
   }
-  float scale_top = vs[0];
+  // From a lane's probabilities (2^15 at most) to what enters the product: times value scale and this, a power of two of at most 2^126 (t is above any score
+  // + log2 scale), below 2^-126 only where scales are 2^96 and more.
+  float to_p[NR][2];
 #pragma unroll
-  for (int b = 1; b < TB; ++b) scale_top = fmaxf(scale_top, vs[b]);
-  if (scale_top > st.ref) {  // the same in all lanes
-    const float inv = inverse_of(scale_top), turn = st.ref * inv;
-    st.ref = scale_top, st.inv = inv;
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-      for (int t = 0; t < S::MT; ++t) st.o[n][t][0] *= turn, st.o[n][t][1] *= turn, st.o[n][t][2] *= turn, st.o[n][t][3] *= turn;
-  }
+    for (int i = 0; i < 2; ++i) to_p[n][i] = ex2_small(st.m[n][i] - st.t[n][i]);
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
-    const float share = vs[b] * st.inv * 32768.f;  // what the probabilities of the block are multiplied by: at most 2^15
     uint32_t hi[NR][2], lo[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -388,9 +397,9 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
         float x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          x[i] = ex2(fmaf(s[b][n][2 * h + i], f[b][n][i], -st.m[n][i]));
+          x[i] = ex2(fmaf(s[b][n][2 * h + i], f[b][n][i], 15.f - st.m[n][i]));
           st.l[n][i] += x[i];
-          x[i] *= share;
+          x[i] *= fminf(vs[b] * to_p[n][i], 3e38f);  // (finite where a scale has no weight: 0 stays 0)
         }
         hi[n][h] = pack_half(x[0], x[1]);
         if constexpr (F32) lo[n][h] = transpose8(rest_half(x[0], x[1], hi[n][h]));
@@ -847,13 +856,17 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
     }
     place += (uint32_t)n_tiles;
 
-    // what brings the output to its own scale and to the maximum of all warps; sums over the eight lanes of a row
-    float unit[NR][2], l[NR][2], m[NR][2];
+    // sums over the eight lanes of a row, and over the warps along the keys; outputs as means of what this block has seen (a mean is no larger than the
+    // largest value, a sum may be)
+    float l[NR][2], m[NR][2];
 #pragma unroll
     for (int j = 0; j < NR; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        l[j][i] = st.l[j][i], m[j][i] = st.m[j][i], unit[j][i] = st.unit();
+        m[j][i] = st.m[j][i];
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) m[j][i] = fmaxf(m[j][i], __shfl_xor_sync(0xffffffffu, m[j][i], o));
+        l[j][i] = st.l[j][i] * ex2(st.m[j][i] - m[j][i]);
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], o);
       }
@@ -875,14 +888,20 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
         l[j][0] = l[j][1] = 0.f;
 #pragma unroll
         for (int k = 0; k < WK; ++k) l[j][0] += x[k].y * ex2(x[k].x - m[j][0]), l[j][1] += x[k].w * ex2(x[k].z - m[j][1]);
-        unit[j][0] *= ex2(st.m[j][0] - m[j][0]), unit[j][1] *= ex2(st.m[j][1] - m[j][1]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float inv = l[j][i] == 0.f ? 0.f : 1.f / l[j][i], up = ex2(st.t[j][i] - m[j][i]);  // (one after the other: their product may be too small)
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
-          st.o[j][t][0] *= unit[j][0], st.o[j][t][1] *= unit[j][1];
-          st.o[j][t][2] *= unit[j][0], st.o[j][t][3] *= unit[j][1];
+          st.o[j][t][i] = st.o[j][t][i] * inv * up;
+          st.o[j][t][2 + i] = st.o[j][t][2 + i] * inv * up;
         }
-        unit[j][0] = unit[j][1] = 1.f;
       }
+    if constexpr (WK > 1) {
       // Half of the warps hand their outputs to the other half, twice: the second time in the place that the giver has read itself.  A lane has rows
       // 2c and 2c + 1 of each eight: where a block never has more than two (or four, six), only lanes of c = 0 (1, 2) have any.
       const int columns = WR == 1 && NR == 1 ? p.region / (S::MT * 16 * 8) : 4;
@@ -916,12 +935,11 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
         for (int i = 0; i < 2; ++i) {
           const int row = row0 + 8 * j + 2 * c + i;
           if (row > last) continue;
-          const float f = part < 0 ? (l[j][i] == 0.f ? 0.f : unit[j][i] / l[j][i]) : unit[j][i];
           const size_t part_row = (size_t)part * L::RB + row;
           const size_t to = (part < 0 ? out_at(p, rows, row) : part_row * DH) + r * (DH / 8);
 #pragma unroll
           for (int t = 0; t < S::MT; t += 2) {
-            const float x[4] = {st.o[j][t][i] * f, st.o[j][t][2 + i] * f, st.o[j][t + 1][i] * f, st.o[j][t + 1][2 + i] * f};
+            const float x[4] = {st.o[j][t][i], st.o[j][t][2 + i], st.o[j][t + 1][i], st.o[j][t + 1][2 + i]};
             if (part < 0)
               store4<F32>(p.out, to + 2 * t, x[0], x[1], x[2], x[3]);
             else
@@ -935,8 +953,8 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
   }
 }
 
-// Joins the parts of the units that lie in several runs, in the order of the keys: m = max m_k, o = sum o_k 2^(m_k - m) / sum l_k 2^(m_k - m).
-// grid: entries, key/value heads, eights of rows.
+// Joins the parts of the units that lie in several runs, in the order of the keys.  A part has the mean o_k of its values, its maximum m_k and its sum l_k:
+// the whole is the mean of the means, weighed by l_k 2^(m_k - m), m = max m_k.  grid: entries, key/value heads, eights of rows.
 template <bool F32, int RB>
 __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   pdl_begin();
@@ -954,17 +972,20 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
     const int row = row0 + i / quads, d = i % quads * 4;
     float m = NOTHING, l = 0.f;
     for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[part_row(k, row) * 2]);
+    for (int k = 0; k < parts; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(k, row) * 2);
+      l += ml.y * ex2(ml.x - m);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < parts; ++k) {
       const size_t at = part_row(k, row);
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float f = ex2(ml.x - m);
+      const float f = ml.y * ex2(ml.x - m) * inv;
       const float4 a = *reinterpret_cast<const float4*>(p.part_o + at * p.head_dim + d);
-      l += ml.y * f;
       o.x += a.x * f, o.y += a.y * f, o.z += a.z * f, o.w += a.w * f;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store4<F32>(p.out, out_at(p, rows, row) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    store4<F32>(p.out, out_at(p, rows, row) + d, o.x, o.y, o.z, o.w);
   }
 }
 

@@ -10,9 +10,10 @@
 // Tensor memory: two tiles of scores, 128 columns each, and two outputs of head dim columns.
 //
 // Scales as in kv8_attention.cuh: a block of 16 keys is 16 columns of the scores, so a key scale is a factor of 16 columns' exponents and a value
-// scale one of their probabilities.  The output stays in tensor memory and is multiplied only when a row's maximum has grown by more
-// than 2^8 since it was last (probabilities are at most 2^8 then) or a value scale exceeds the reference; probabilities times share are at
-// most 2^15 and keep 11 bits down to 2^-14.
+// scale one of their probabilities, which are held as halves of 2^(score + log2 scale - m - u).  m: the row's maximum, which follows when it has grown by
+// more than 2^8; m + u goes with T there, the largest score + log2 scale that the row has seen: the output stays in tensor memory and is multiplied
+// only when T would put a half above 2^15, and then T stands at 2^11.  So the key that moves the output most stands between 2^10 and 2^15, keys down to
+// 2^-24 of it keep all of their 11 bits, and none is off by more than 2^-35 of it.
 //
 // What bounds it: 128 x 128 exponentials take 1024 cycles of an SM, the products of a tile 1024 (head 128) or 512; turning 32 KB of codes into
 // halves takes 260 issue slots a scheduler.  Work is shared over the SMs in equal runs of tiles, as there.  Measured: a tile takes 3,350 cycles at
@@ -36,7 +37,7 @@ struct TcLayout {
   static constexpr int Q = 0, K = MAT, V = K + 2 * MAT;
   static constexpr int NAN_BITS = V + 2 * MAT;         // [stage][key][DH / 16] a bit for each value of a tile that not every row sees whole: NaN
   static constexpr int NAN_SOME = NAN_BITS + 2 * TC_KEYS * (DH / 8);  // [stage][8 warps]: whether there is one
-  static constexpr int ML = NAN_SOME + 2 * 8 * 4;      // [group][128 rows] maximum, sum, reference, whether there is anything
+  static constexpr int ML = NAN_SOME + 2 * 8 * 4;      // [group][128 rows] maximum, sum, u + 11, whether there is anything
   static constexpr int FACTOR = ML + 2 * 128 * 16;     // [128 rows]
   static constexpr int SEG = FACTOR + 512;             // two segments
   static constexpr int BARS = SEG + 2 * 64;
@@ -397,7 +398,8 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       meet();
       if (lane == 0) arrive(bar(Q_READY));
       if (g == 1) factor = factors[row];
-      float m = NOTHING, l = 0.f, ref = 0.f;
+      float m = NOTHING, l = 0.f, t = NOTHING;  // maximum, sum of 2^(score - m), largest score + log2(value scale)
+      int u = 0;
       uint32_t bad[DH / 32] = {};  // dims that a NaN value in this row's sight has
       bool any_bad = false;
       // scales: lanes 0 to 7 of a tile's blocks of keys, 8 to 15 of values; pages a tile of this group ahead of that
@@ -420,24 +422,23 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         const bool there = __all_sync(0xffffffffu, lane >= 8 || scale >= 0.f);
         const bool whole = there && is_whole(s, key0);
         // of the eight blocks: what scores are multiplied by, and the value scales' exponents
-        float f[8], share_top = 0.f;
+        float f[8];
         int ve[8];
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
           const float ks = __shfl_sync(0xffffffffu, scale, b), vs = __shfl_sync(0xffffffffu, scale, 8 + b);
           f[b] = factor * ks;
-          ve[b] = (int)(__float_as_uint(vs) >> 23) + 7;
-          share_top = fmaxf(share_top, vs);
+          ve[b] = (int)(__float_as_uint(vs) >> 23) - 127;
         }
         ok = wait(S_FULL + g, s_count & 1u);
         if (!ok) break;
         ++s_count;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (some_row) {
-          // the tile's maximum, in units of log 2
+          // the tile's maxima, in units of log 2
           // (columns from lo_vis to hi_vis - 1 are of keys that the row sees)
           const int hi_vis = qpos - key0 + 1, lo_vis = p.window > 0 ? qpos - p.window + 1 - key0 : 0;
-          float top = NOTHING;
+          float top = NOTHING, top_t = NOTHING;
           uint32_t ra[32], rb[32];  // two blocks' columns each, one on its way while the other is used
           auto most_of = [&](const uint32_t(&x)[32], int b) {
 #pragma unroll
@@ -445,7 +446,9 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
               float y[2] = {NOTHING, NOTHING};
 #pragma unroll
               for (int k = 0; k < 16; k += 2) y[k / 2 & 1] = max3(y[k / 2 & 1], __uint_as_float(x[16 * h + k]), __uint_as_float(x[16 * h + k + 1]));
-              top = fmaxf(top, fmaxf(y[0], y[1]) * f[b + h]);
+              const float z = fmaxf(y[0], y[1]) * f[b + h];
+              top = fmaxf(top, z);
+              top_t = fmaxf(top_t, z + (float)ve[b + h]);
             }
           };
           if (whole) {
@@ -465,6 +468,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
 #pragma unroll 1
             for (int b = 0; b < 8; b += 2) {
               const float k0 = __shfl_sync(0xffffffffu, scale, b), k1 = __shfl_sync(0xffffffffu, scale, b + 1);
+              const float v0 = __shfl_sync(0xffffffffu, scale, 8 + b), v1 = __shfl_sync(0xffffffffu, scale, 9 + b);
               tc::tmem_load32(s_at + 16u * b, ra);
               tmem_wait_load(ra);
 #pragma unroll
@@ -474,16 +478,19 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
                 float y = NOTHING;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) y = k >= lo && k < hi ? fmaxf(y, __uint_as_float(ra[16 * h + k])) : y;
-                top = y == NOTHING ? top : fmaxf(top, y * (factor * ks));
+                const float z = y == NOTHING ? NOTHING : y * (factor * ks);
+                top = fmaxf(top, z);
+                top_t = fmaxf(top_t, z + (float)((int)(__float_as_uint(h ? v1 : v0) >> 23) - 127));
               }
             }
           }
-          // the output follows when the maximum has grown by more than 2^8, or a value scale is above the reference
-          const float m_new = top > m + 8.f || m == NOTHING ? fmaxf(m, top) : m;
-          const float ref_new = share_top > ref ? 2.f * share_top : ref;
-          if (__any_sync(0xffffffffu, m_new != m || ref_new != ref)) {
-            const float turn_l = ex2(m - m_new), turn = turn_l * (ref == 0.f ? 0.f : ref * inverse_of(ref_new));
-            l *= turn_l;
+          t = fmaxf(t, top_t);
+          const bool up = top > m + 8.f || m == NOTHING;
+          const float m_new = up ? fmaxf(m, top) : m;
+          const int u_new = up || t - m_new > (float)(u + 15) ? (int)ceilf(t - m_new) - 11 : u;
+          if (__any_sync(0xffffffffu, m_new != m || u_new != u)) {
+            const float turn = ex2(m - m_new + (float)(u - u_new));
+            l *= ex2(m - m_new);
             if (!first) {
               ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
               if (ok) {
@@ -500,7 +507,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
               }
             }
-            m = m_new, ref = ref_new;
+            m = m_new, u = u_new;
           }
           // The groups take turns at what follows, tile by tile: side by side they would both wait for the exponentials and then both for the products.
           if (ok && i > 0) ok = wait(WEIGHED + (1 - g), (others + (uint32_t)(i - 1) / 2u) & 1u);
@@ -508,14 +515,13 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
             ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
-          // Probabilities times share, over the scores that have been read: the share is a power of two and goes into the exponent (2^-60 at
-          // least: what lies below adds nothing to a half), and the sum of a block's is brought back by it.
-          const int ref_e = (int)(__float_as_uint(ref) >> 23);
+          // Probabilities times value scale, over the scores that have been read: the scale is a power of two and goes into the exponent (from 2^-60 on:
+          // what lies below adds nothing to a half), and the sum of a block's is brought back by it.
           auto weigh = [&](const uint32_t(&x)[32], int b) {
             uint32_t packed[16];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int e = max(ve[b + h] - ref_e, -60);
+              const int e = max(ve[b + h] - u, -60);
               const float from = (float)e - m;
               const uint64_t f2 = pair(f[b + h], f[b + h]), from2 = pair(from, from);
               uint64_t sum2[2] = {0ull, 0ull};
@@ -527,7 +533,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
                 packed[8 * h + k / 2] = pack_half(x0, x1);
               }
               const uint64_t both = add2(sum2[0], sum2[1]);
-              l = fmaf(__uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32)), __uint_as_float((uint32_t)(127 - e) << 23), l);
+              l = fmaf(__uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32)), __uint_as_float((uint32_t)max(127 - e, 0) << 23), l);
             }
             tmem_store16(p_at + 8u * b, packed);
           };
@@ -556,7 +562,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
               for (int h = 0; h < 2; ++h) {
                 const float ks = h ? k1 : k0, by = factor * ks;
                 const int lo = lo_vis - (b + h) * BLOCK, hi = ks < 0.f ? 0 : hi_vis - (b + h) * BLOCK;
-                const int e = max((int)(__float_as_uint(h ? v1 : v0) >> 23) + 7 - ref_e, -60);
+                const int e = max((int)(__float_as_uint(h ? v1 : v0) >> 23) - 127 - u, -60);
                 const float from = (float)e - m;
                 float sum = 0.f;
 #pragma unroll
@@ -567,7 +573,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
                   sum += x0 + x1;
                   packed[8 * h + k / 2] = pack_half(x0, x1);
                 }
-                l = fmaf(sum, __uint_as_float((uint32_t)(127 - e) << 23), l);
+                l = fmaf(sum, __uint_as_float((uint32_t)max(127 - e, 0) << 23), l);
               }
               tmem_store16(p_at + 8u * b, packed);
             }
@@ -604,7 +610,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       others += (uint32_t)(s.n_tiles + g) / 2u;
       // the unit's end: both groups' outputs, each group half of the columns
       if (ok && !first) ok = wait(PV_DONE + g, (pv_count - 1u) & 1u);
-      ml[g * 128 + row] = make_float4(m, l, ref, first ? 0.f : 1.f);
+      ml[g * 128 + row] = make_float4(m, l, (float)(u + 11), first ? 0.f : 1.f);
       uint32_t* bad_at = reinterpret_cast<uint32_t*>(smem + L::Q) + row * (DH / 32);  // [group][row]: the queries are used
       const bool bad_somewhere = !all_of_us(!any_bad);
       if (bad_somewhere) {
@@ -616,8 +622,8 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
       if (ok && some_row) {
         const float4 a = ml[row], b = ml[128 + row];
         const float top = fmaxf(a.x, b.x), fa = ex2(a.x - top), fb = ex2(b.x - top), sum = a.y * fa + b.y * fb;
-        const float scale = s.part < 0 ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-        const float ua = fa * scale * (a.z * 0.0078125f), ub = fb * scale * (b.z * 0.0078125f);  // ref * 2^-7
+        // means (which are no larger than the largest value; a sum may be); the powers of two in halves, of which neither is too small or too large
+        const float by = sum == 0.f ? 0.f : 4.8828125e-4f / sum, ua = ex2(0.5f * (a.x - top + a.z)), ub = ex2(0.5f * (b.x - top + b.z));  // 2^-11
         const size_t part_row = (size_t)s.part * TC_ROWS + row;
         const size_t to = s.part < 0 ? (size_t)(s.token0 + q) * p.out_stride + (size_t)h * DH : part_row * DH;
 #pragma unroll 1
@@ -629,7 +635,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
           tmem_wait_load(rb);
           float o[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = (a.w != 0.f ? __uint_as_float(ra[k]) * ua : 0.f) + (b.w != 0.f ? __uint_as_float(rb[k]) * ub : 0.f);
+          for (int k = 0; k < 32; ++k) o[k] = (a.w != 0.f ? __uint_as_float(ra[k]) * by * ua * ua : 0.f) + (b.w != 0.f ? __uint_as_float(rb[k]) * by * ub * ub : 0.f);
           if (bad_somewhere) {
             const uint32_t word = bad_at[c / 32] | bad_at[128 * (DH / 32) + c / 32];
 #pragma unroll

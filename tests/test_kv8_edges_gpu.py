@@ -64,3 +64,95 @@ def test_queries_of_the_largest_size(K, dtype, each):
 
     T.check_attention(K, each, 2, 2, 64, 16, dtype, touch=touch)
     assert on_tcgen05(K, each, 2, 2, 64, 16) == (each[0][1] == 70)
+
+
+# ---- values of very different sizes ----------------------------------------------------------------
+
+def blocks_of(batch, r):
+    """(block of 16 keys, page, block of the page) of a request."""
+    for b in range(-(-batch.each[r][0] // 16)):
+        page, row = batch.row_of(r, b * 16)
+        yield b, page, row // 16
+
+
+def apart(shift, down, every=3):
+    """Keys of every third block score ``shift`` (nats) lower than the others, and values of the other blocks are 2^-down of theirs."""
+    def touch(batch, q, pool, scales):
+        dim, n_kv = pool.shape[4], pool.shape[2]
+        heads = q.shape[1] // dim
+        q.view(batch.tokens, heads, dim)[:, :, 0] = 8.0
+        low = torch.tensor(-shift * dim ** 0.5 / 8.0 / 0.25).to(torch.float8_e4m3fn).view(torch.uint8)
+        codes = pool.view(torch.uint8)
+        for r in range(len(batch.each)):
+            for b, page, sub in blocks_of(batch, r):
+                rows = slice(16 * sub, 16 * sub + 16)
+                if b % every == 0:
+                    codes[page, 0, :, rows] = 0
+                    codes[page, 0, :, rows, 0] = low
+                    scales[page, 0, :, sub] = 0.25
+                else:
+                    codes[page, 0, :, rows, 0] = 0
+                    scales[page, 1, :, sub] *= 2.0 ** -down
+
+    return touch
+
+
+# a unit a block, shares that are joined, few queries, many, in 32 bits; tcgen05 with heads of 64 and 128 and in shares
+SHAPES = [([(700, 1), (90, 1)], 2, 2, 64, 16, BF16), ([(3000, 1), (40, 1)], 4, 1, 64, 32, BF16), ([(300, 5), (33, 1)], 4, 1, 128, 16, BF16),
+          ([(300, 100)], 1, 1, 96, 16, BF16), ([(700, 1), (200, 60)], 2, 2, 64, 16, F32), ([(2500, 4)], 2, 1, 256, 64, F32),
+          ([(700, 130), (20, 1)], 2, 2, 64, 16, BF16), ([(900, 70)], 4, 2, 128, 64, BF16)]
+
+
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("shift,down", [(40, 12), (40, 20), (40, 24), (40, 32), (60, 60), (26, 50), (26, 90), (0, 40)])
+def test_values_of_very_different_sizes(K, shape, shift, down):
+    """What a row weighs most may lie in blocks whose values are the smallest in its sight, or the product of a tiny probability and a huge value: every
+    entry is within the bound of its own sum of probabilities times values."""
+    each, heads, n_kv, dim, page, dtype = SHAPES[shape]
+    assert on_tcgen05(K, each, heads, n_kv, dim, page) == (shape >= 6)
+    T.check_attention(K, each, heads, n_kv, dim, page, dtype, spread=0.0, touch=apart(shift, down))
+
+
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_values_of_nothing_beside_others(K, shape):
+    """Blocks whose values are all zero (their scale is the smallest) beside ordinary ones."""
+    def touch(batch, q, pool, scales):
+        for r in range(len(batch.each)):
+            for b, page, sub in blocks_of(batch, r):
+                if b % 2 == 0:
+                    rows = slice(16 * sub, 16 * sub + 16)
+                    codes = pool.view(torch.uint8)
+                    codes[page, 1, :, rows] = torch.where(codes[page, 1, :, rows] == 0x7F, codes[page, 1, :, rows], 0)  # (NaN behind the last token stays)
+                    scales[page, 1, :, sub] = 2.0 ** -126
+
+    each, heads, n_kv, dim, page, dtype = SHAPES[shape]
+    T.check_attention(K, each, heads, n_kv, dim, page, dtype, touch=touch)
+
+
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_values_of_the_largest_size(K, shape):
+    """Means of values near the largest finite one are finite."""
+    def touch(batch, q, pool, scales):
+        scales[:, 1] = 2.0 ** 119  # codes of up to 448
+
+    each, heads, n_kv, dim, page, dtype = SHAPES[shape]
+    got = T.check_attention(K, each, heads, n_kv, dim, page, dtype, touch=touch)
+    assert torch.isfinite(got).all() and got.abs().max() > 1e37
+
+
+@pytest.mark.parametrize("up", [20, 31, 60, 125])
+@pytest.mark.parametrize("each,heads,n_kv,dim,dtype", [([(160, 100)], 2, 2, 64, BF16), ([(160, 100)], 3, 1, 32, BF16), ([(96, 40)], 2, 1, 64, F32), ([(640, 200)], 2, 1, 64, BF16),
+                                                       ([(1024, 150)], 2, 2, 128, BF16)])
+def test_a_value_that_a_row_does_not_see_changes_nothing_for_it(K, each, heads, n_kv, dim, dtype, up):
+    """The values of one block, that some rows see and others do not, become 2^up times as large: the rows ahead of it keep every bit, the others are right."""
+    n, nq = each[0]
+    block = (n - nq // 3) // 16
+    outs = []
+    for by in (0, up):
+        def touch(batch, q, pool, scales):
+            page, row = batch.row_of(0, 16 * block)
+            scales[page, 1, :, row // 16] = 2.0 ** (by - 6)
+
+        outs.append(T.check_attention(K, each, heads, n_kv, dim, 16, dtype, touch=touch))
+    ahead = 16 * block - (n - nq)
+    assert 0 < ahead < nq and outs[0][:ahead].equal(outs[1][:ahead]) and not outs[0][ahead:].equal(outs[1][ahead:])
