@@ -15,12 +15,11 @@
 //
 // Scales: the 16 keys of a block share a key scale, by which their scores are multiplied.  A block of values is one inner step of P V, so its
 // probabilities are multiplied by its scale.  The outputs therefore have a maximum of their own beside the softmax's: T, the largest score + log2(value
-// scale) that the row has seen, rounded up; probabilities enter P V as halves of 2^(score + log2 scale - T + 15).  The key that moves the output most thus
-// stands between 2^14 and 2^15 whatever the scales are, keys down to 2^-29 of it keep all of their 11 bits (relative error 2^-11, against 2^-8 of a
-// bfloat16 output), and none is off by more than 2^-40 of it.  What a row does not see has no part in T.  (Probabilities against the largest scale so
-// far, which may belong to keys of no weight or out of sight, lost bits from a ratio of 2^-18 on and everything at 2^-40.)  The
-// sum of the probabilities needs no row's maximum: each lane has its own for its own keys.  Both maxima are whole numbers, so that all changes of them are exact.
-// Q is brought to halves row by row with a power of two that puts its largest entry at 2^14 (a bfloat16 fits exactly,
+// scale) that the row has seen; probabilities enter P V as halves of 2^(score + log2 scale - T + 15).  The key that moves the output most thus
+// stands at 2^15 (exactly, where it alone matters) whatever the scales are, keys down to 2^-29 of it keep all of their 11 bits (relative error 2^-11, against
+// 2^-8 of a bfloat16 output), and none is off by more than 2^-40 of it.  What a row does not see has no part in T.  (Probabilities against the largest
+// scale so far, which may belong to keys of no weight or out of sight, lost bits from a ratio of 2^-18 on and everything at 2^-40.)  In 32 bits T is
+// rounded up: changes of it are exact then.  Q is brought to halves row by row with a power of two that puts its largest entry at 2^14 (a bfloat16 fits exactly,
 // within 2^-28 of the row's largest); in 32 bits Q and P are two halves each, a value and what its rounding left, so that products
 // are exact to 2^-22.  Sums, maxima and outputs are float32.
 #pragma once
@@ -256,13 +255,14 @@ constexpr float NOTHING = -1.7e38f;  // the maximum of no score: finite, so that
 template <int DH, int NR>
 struct State {
   float o[NR][DH / 16][4];  // tile i: entries [0], [1] are dim r * DH / 8 + 2 i of the two rows (r = lane / 4), [2], [3] the dim after it
-  float t[NR][2];           // the rows' largest score + log2(value scale), in units of log 2, rounded up; o is the sum of 2^(score - t + 15) * v
-  float m[NR][2], l[NR][2]; // the largest score of this lane's keys, rounded up, and the sum of 2^(score - m + 15) over them
+  float t[NR][2];           // the largest score + log2(value scale), in units of log 2; o is the sum of 2^(score - t + 15) * v
+  float to_p[NR][2];        // 2^(15 + m - t): from a probability times its value scale to what enters the product
+  float m[NR][2], l[NR][2]; // maximum (in units of log 2) and sum of 2^(score - m); the sum is over this lane's keys only until the end
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) t[n][i] = m[n][i] = NOTHING, l[n][i] = 0.f;
+      for (int i = 0; i < 2; ++i) t[n][i] = m[n][i] = NOTHING, l[n][i] = to_p[n][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < DH / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -340,28 +340,29 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
           f[b][n][i] = 1.f;
         }
   }
-  float lv[TB];  // log2 of the value scales
 #pragma unroll
-  for (int b = 0; b < TB; ++b) lv[b] = (float)((int)(__float_as_uint(vs[b]) >> 23) - 127);
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[n][i] = NOTHING;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) top[n][i] = fmaxf(top[n][i], fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i]);
+    }
+  // log2 of a value scale (its exponent as the low bits of a float); from 2^-111 on, so that 2^(15 + m - t) is a float
+  auto log_of = [](float v) { return fmaxf(__uint_as_float(0x4B000000u | (__float_as_uint(v) >> 23)) - 8388735.f, -111.f); };
+  float scale_top = vs[0];
+#pragma unroll
+  for (int b = 1; b < TB; ++b) scale_top = fmaxf(scale_top, vs[b]);
+  const float log_top = log_of(scale_top);
   bool grown = false;
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float own = NOTHING;
-      top[n][i] = NOTHING;
-#pragma unroll
-      for (int b = 0; b < TB; ++b) {
-        const float y = fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i];
-        own = fmaxf(own, y);
-        top[n][i] = fmaxf(top[n][i], y + lv[b]);
-      }
-      const float m = fmaxf(st.m[n][i], ceilf(own));
-      st.l[n][i] *= ex2(st.m[n][i] - m);
-      st.m[n][i] = m;
 #pragma unroll
       for (int o = 4; o < 32; o *= 2) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], o));
-      grown |= top[n][i] > st.t[n][i];
+      // (the largest score and the largest scale may be of different keys: whether t grows is looked at below)
+      grown |= top[n][i] > st.m[n][i] || top[n][i] + log_top > st.t[n][i];
     }
   if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -369,9 +370,17 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
       float turn[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float t = fmaxf(st.t[n][i], ceilf(top[n][i]));
+        float t = NOTHING;
+#pragma unroll
+        for (int b = 0; b < TB; ++b) t = fmaxf(t, fmaxf(s[b][n][i], s[b][n][2 + i]) * f[b][n][i] + log_of(vs[b]));
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+        t = fmaxf(st.t[n][i], F32 ? ceilf(t) : t);
+        const float m = fmaxf(st.m[n][i], top[n][i]);
+        st.l[n][i] *= ex2(st.m[n][i] - m);
         turn[i] = ex2(st.t[n][i] - t);
-        st.t[n][i] = t;
+        st.m[n][i] = m, st.t[n][i] = t;
+        st.to_p[n][i] = ex2_small(15.f + (m - t));
       }
 #pragma unroll
       for (int t = 0; t < S::MT; ++t) {
@@ -380,13 +389,6 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
       }
     }
   }
-  // From a lane's probabilities (2^15 at most) to what enters the product: times value scale and this, a power of two of at most 2^126 (t is above any score
-  // + log2 scale), below 2^-126 only where scales are 2^96 and more.
-  float to_p[NR][2];
-#pragma unroll
-  for (int n = 0; n < NR; ++n)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) to_p[n][i] = ex2_small(st.m[n][i] - st.t[n][i]);
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
     uint32_t hi[NR][2], lo[NR][2];
@@ -397,9 +399,9 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
         float x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          x[i] = ex2(fmaf(s[b][n][2 * h + i], f[b][n][i], 15.f - st.m[n][i]));
+          x[i] = ex2(fmaf(s[b][n][2 * h + i], f[b][n][i], -st.m[n][i]));
           st.l[n][i] += x[i];
-          x[i] *= fminf(vs[b] * to_p[n][i], 3e38f);  // (finite where a scale has no weight: 0 stays 0)
+          x[i] = x[i] * vs[b] * st.to_p[n][i];  // (in this order: the two factors' product may be no float where the probability is 0)
         }
         hi[n][h] = pack_half(x[0], x[1]);
         if constexpr (F32) lo[n][h] = transpose8(rest_half(x[0], x[1], hi[n][h]));
@@ -821,7 +823,11 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
 #pragma unroll
     for (int j = 0; j < NR; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) factor[j][i] = factors[8 * j + 2 * c + i], pos[j][i] = position(row0 + 8 * j + 2 * c + i);
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + 8 * j + 2 * c + i;
+        factor[j][i] = row <= last ? factors[8 * j + 2 * c + i] : 0.f;  // (rows behind the last one: scores that never grow)
+        pos[j][i] = position(row);
+      }
     const int pos_lo = position(row0), pos_hi = position(row0 + L::RW - 1);
     slot = (place + (uint32_t)wk) % n_ring, phase = ((place + (uint32_t)wk) / n_ring) & 1u;
     for (int i = wk; i < n_tiles && ok; i += WK) {
@@ -863,10 +869,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
     for (int j = 0; j < NR; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        m[j][i] = st.m[j][i];
-#pragma unroll
-        for (int o = 4; o < 32; o *= 2) m[j][i] = fmaxf(m[j][i], __shfl_xor_sync(0xffffffffu, m[j][i], o));
-        l[j][i] = st.l[j][i] * ex2(st.m[j][i] - m[j][i]);
+        m[j][i] = st.m[j][i], l[j][i] = st.l[j][i];
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], o);
       }
@@ -894,7 +897,8 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
     for (int j = 0; j < NR; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float inv = l[j][i] == 0.f ? 0.f : 1.f / l[j][i], up = ex2(st.t[j][i] - m[j][i]);  // (one after the other: their product may be too small)
+        // (2^-15 / l and 2^(t - m) one after the other: their product may be too small)
+        const float inv = l[j][i] == 0.f ? 0.f : 3.0517578125e-05f / l[j][i], up = ex2(st.t[j][i] - m[j][i]);
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
           st.o[j][t][i] = st.o[j][t][i] * inv * up;
@@ -971,10 +975,11 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   for (int i = threadIdx.x; i < n_rows * quads; i += 128) {
     const int row = row0 + i / quads, d = i % quads * 4;
     float m = NOTHING, l = 0.f;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[part_row(k, row) * 2]);
     for (int k = 0; k < parts; ++k) {
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(k, row) * 2);
-      l += ml.y * ex2(ml.x - m);
+      const float most = fmaxf(m, ml.x);
+      l = l * ex2(m - most) + ml.y * ex2(ml.x - most);
+      m = most;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
