@@ -232,10 +232,11 @@ struct Queries {
 #pragma unroll
       for (int k = 0; k < DH / 32; ++k) top = fmaxf(top, fabsf(x[n][k]));
       top = warp_max(top);
-      // the power of two that puts the largest entry between 2^14 and 2^15 (kept within the exponents for which both factors are normal numbers)
+      // the power of two that puts the largest entry between 2^14 and 2^15, with the sign of the scale: factors are positive, and the largest score is the
+      // largest product (kept within the exponents for which both factors are normal numbers)
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 127);
-      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23), down = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-      if (lane == 0) factor[r] = down * p.scale * 1.4426950408889634f;
+      const float up = copysignf(__uint_as_float((uint32_t)(14 - e + 127) << 23), p.scale), down = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      if (lane == 0) factor[r] = down * fabsf(p.scale) * 1.4426950408889634f;
 #pragma unroll
       for (int k = 0; k < DH / 32; ++k) {
         const int d = lane + 32 * k, c = d / S::CHUNK % 4, step = d / (4 * S::CHUNK) * (S::CHUNK / 4) + d % S::CHUNK / 4;

@@ -382,8 +382,8 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
           for (int k = 0; k < 4; ++k) top = max3(top, fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xFFFF0000u)));
         }
         const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -110), 127);
-        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * p.scale * 1.4426950408889634f;
+        const float up = copysignf(__uint_as_float((uint32_t)(14 - e + 127) << 23), p.scale);  // (the sign of the scale, so that factors are positive)
+        factor = __uint_as_float((uint32_t)(e - 14 + 127) << 23) * fabsf(p.scale) * 1.4426950408889634f;
 #pragma unroll
         for (int c = 0; c < DH / 8; ++c) {
           const uint32_t u[4] = {w[c].x, w[c].y, w[c].z, w[c].w};

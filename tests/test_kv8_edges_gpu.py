@@ -66,6 +66,26 @@ def test_queries_of_the_largest_size(K, dtype, each):
     assert on_tcgen05(K, each, 2, 2, 64, 16) == (each[0][1] == 70)
 
 
+@pytest.mark.parametrize("scale", [-0.125, -1.0, 0.0])
+@pytest.mark.parametrize("dtype,each,dim", [(F32, [(200, 1), (150, 40)], 64), (BF16, [(2300, 1), (150, 20)], 96), (BF16, [(600, 70), (40, 1)], 64), (BF16, [(600, 130)], 128)])
+def test_scales_that_are_not_positive(K, dtype, each, dim, scale):
+    """The smallest product is the largest score then; with none, all keys in sight weigh the same."""
+    gen = torch.Generator().manual_seed(13)
+    batch = P.Batch(each, 16, seed=13)
+    pool, scales = T.cache_of(batch, 2, dim, gen)
+    q = (torch.randn(batch.tokens, 2 * dim, generator=gen) * 1.5).to(dtype)
+    want = list(P.attention(batch, q.double().unflatten(1, (2, dim)), P.values_of(pool), scales.double(), 2, scale))
+    if scale < 0:  # the bounds for a scale of that size
+        want[1:] = P.attention(batch, -q.double().unflatten(1, (2, dim)), P.values_of(pool), scales.double(), 2, -scale)[1:]
+    a = batch.arrays(DEV)
+    out = torch.full((batch.tokens, 2 * dim), 7.0, dtype=dtype, device=DEV)
+    K.kv8_attention(q.to(DEV), pool.to(DEV), scales.to(DEV), a["block_table"], a["q_start"], a["kv_len"], a["slots"], out, n_heads=2, scale=scale,
+                    span=max(n for n, _ in each), tiles=a["tiles"], n_tiles=len(batch.tiles), max_q=max(n for _, n in each), decode_reqs=a["decode_reqs"],
+                    n_decode=len(batch.single))
+    K.check_status(DEV)
+    T.compare(out, *want, dtype)
+
+
 # ---- values of very different sizes ----------------------------------------------------------------
 
 def blocks_of(batch, r):
