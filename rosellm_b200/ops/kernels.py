@@ -2183,6 +2183,7 @@ def kv8_write(k, v, pool, scales, block_table, positions, req_of_token, q_start,
 
 
 _KV8_PLANS: dict[tuple, tuple[int, int, int, int, int, int]] = {}
+_KV8_PLANS_KEPT = 4096
 
 
 def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int, n_kv: int, dh: int, page_size: int, span: int) -> tuple[int, int, int, int, int, int]:
@@ -2191,31 +2192,29 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
 
     SMs 0: every unit (an item's rows for one key/value head) has a block to itself; else all keys are shared evenly by as many blocks as stand on
     the device at once, and what lies in several is joined."""
-    key = (code, is_tiles, n_items, queries, n_heads, n_kv, dh, page_size, span)
+    rows = queries * (n_heads // n_kv)
+    on_tcgen05, by_units = kv8_on_tcgen05(code, rows, dh, page_size, span), _kv8_by_units(dh, span)
+    key = (code, is_tiles, n_items, queries, n_heads, n_kv, dh, on_tcgen05, by_units)  # (a span of its own at every step: kept by what follows from it)
     have = _KV8_PLANS.get(key)
     if have is not None:
         return have
-    rows = queries * (n_heads // n_kv)
-    block = 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
-    if kv8_on_tcgen05(code, rows, dh, page_size, span):
-        block = 128
+    block = 128 if on_tcgen05 else 8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 32 else 64
     row_blocks = -(-rows // block)
     entries = n_items * row_blocks
     sms = sm_count()
-    if block == 128 and entries <= KV8_MOST_ENTRIES:
-        plan = -(-(entries + 2) // 4) * 4
-        have = _KV8_PLANS[key] = (block, row_blocks, sms, sms, plan, plan + sms * 2 * block * (dh + 2))
-        return have
-    if block == 128:
+    if block == 128 and entries > KV8_MOST_ENTRIES:
         block, row_blocks = 64, -(-rows // 64)
         entries = n_items * row_blocks
-    at_once = sms * _lib().rl_kv8_attention_blocks(code, block, is_tiles, n_heads, n_kv, dh)
-    if _kv8_by_units(dh, span) or entries > KV8_MOST_ENTRIES:
-        have = (block, row_blocks, 0, 0, 0, 0)
+    if block == 128:
+        at_once = sms
     else:
+        at_once = 0 if by_units or entries > KV8_MOST_ENTRIES else sms * _lib().rl_kv8_attention_blocks(code, block, is_tiles, n_heads, n_kv, dh)
+    if at_once:
         plan = -(-(entries + 2) // 4) * 4
         have = (block, row_blocks, sms, at_once, plan, plan + at_once * 2 * block * (dh + 2))
-    if len(_KV8_PLANS) > 4096:
+    else:
+        have = (block, row_blocks, 0, 0, 0, 0)
+    if len(_KV8_PLANS) >= _KV8_PLANS_KEPT:
         _KV8_PLANS.clear()
     _KV8_PLANS[key] = have
     return have

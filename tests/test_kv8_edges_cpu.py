@@ -28,3 +28,17 @@ def test_a_pool_without_pages_is_refused():
                                          rows, 1, sms, 148, at, at, at, at, None)
 
     assert [attend(128, 148, 0), attend(8, 0, 0), attend(64, 148, -1)] == [-11] * 3
+
+
+def test_plans_that_are_kept_are_few(monkeypatch):
+    """A process whose contexts grow by a token a step, in batches of ever other sizes, keeps a bounded number of plans, the same for contexts that are
+    treated alike."""
+    monkeypatch.setattr(K, "device_facts_given", (148, 233472))
+    monkeypatch.setattr(K, "_KV8_PLANS", {})
+    size = dict(dtype=torch.bfloat16, n_heads=12, n_kv=12, head_dim=64, page_size=16)
+    plans = {K.kv8_attention_plan(span=span, n_tiles=4, max_q=64, n_decode=3, **size) for span in range(512, 20000)}
+    assert len(K._KV8_PLANS) <= 4 and len(plans) <= 2
+    for n in range(1, 6000):
+        K.kv8_attention_plan(span=3000, n_tiles=n, max_q=64, n_decode=n, **size)
+        assert len(K._KV8_PLANS) <= 4096
+    assert K.kv8_attention_plan(span=511, n_tiles=4, max_q=64, **size) != K.kv8_attention_plan(span=512, n_tiles=4, max_q=64, **size)
