@@ -284,14 +284,23 @@ class InferenceEngine:
         """The tokens generated so far that the host has read."""
         return [t for t in self._requests[request_id].output_ids if t != PENDING]
 
+    def _take_away(self, request_id):
+        """The request that the engine will not speak of any more, and no token of it that was read early (its name may be another's by the next step);
+        ``None`` if it knows no such request."""
+        if request_id in self._read_early:
+            self._read_early = {i: t for i, t in self._read_early.items() if i != request_id}
+        return self._requests.pop(request_id, None)
+
     def pop_response(self, request_id) -> RequestOutput:
-        req = self._requests.pop(request_id)
+        if request_id not in self._requests:
+            raise KeyError(request_id)
+        req = self._take_away(request_id)
         text = self.decode(req.output_ids) if self.tokenizer is not None else None
         return RequestOutput(req.request_id, list(req.prompt_ids), list(req.output_ids), req.finish_reason,
                              text, req.num_preemptions)
 
     def discard_request(self, request_id) -> None:
-        req = self._requests.pop(request_id, None)
+        req = self._take_away(request_id)
         if req is not None and req.status != FINISHED:
             self.scheduler.abort(req)
 
@@ -343,7 +352,7 @@ class InferenceEngine:
                 yield text[len(shown):]
                 shown = text
         self.pop_finished_ids()
-        self._requests.pop(rid, None)
+        self._take_away(rid)
 
 
 class LLM:

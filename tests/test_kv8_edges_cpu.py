@@ -1,10 +1,15 @@
 """The 8-bit cache and forks at the ends of their ranges, as far as no device is needed; what only the sources can show."""
 import os
 import re
+from types import SimpleNamespace
 
+import pytest
 import torch
 
+from rosellm_b200.engine.llm import InferenceEngine
 from rosellm_b200.ops import kernels as K
+from rosellm_b200.sampling.params import SamplingParams
+from test_scheduler_cpu import make
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rosellm_b200", "csrc")
 
@@ -42,3 +47,57 @@ def test_plans_that_are_kept_are_few(monkeypatch):
         K.kv8_attention_plan(span=3000, n_tiles=n, max_q=64, n_decode=n, **size)
         assert len(K._KV8_PLANS) <= 4096
     assert K.kv8_attention_plan(span=511, n_tiles=4, max_q=64, **size) != K.kv8_attention_plan(span=512, n_tiles=4, max_q=64, **size)
+
+
+# ---- requests that fork, through the engine's own bookkeeping --------------------------------------
+
+class Engine(InferenceEngine):
+    """The engine's bookkeeping in overlapped mode around a model that is not there: token n of any request is 10 + n."""
+
+    def __init__(self, **kw):
+        self.scheduler, self.cache = make(**kw)
+        self.runner = SimpleNamespace(fork=self.cache.fork, check_status=lambda: None)
+        self.overlap_schedule, self.tokenizer = True, None
+        self._inflight, self._requests, self._finished_ids = None, {}, []
+        self.num_steps = self.num_preemptions = self._since_status_check = 0
+
+    def _launch(self, plan):
+        for item in plan.items:
+            self.cache.commit(item.request.slot, item.count)
+        sampling = [i.request for i in plan.items if i.samples]
+        tokens = [10 + len(r.output_ids) for r in sampling]
+        return sampling, SimpleNamespace(tokens=lambda: tokens)
+
+    def add(self, n=3, request_id=None):
+        return self.add_request(prompt_token_ids=list(range(1, 6)), request_id=request_id, sampling_params=SamplingParams(max_new_tokens=n, stop_on_eos=False))
+
+
+@pytest.mark.parametrize("end", ["discard_request", "pop_response"])
+def test_tokens_read_for_a_fork_are_not_reported_for_a_request_that_is_gone(end):
+    """A fork reads the tokens of the step in flight, which the next call of ``step`` reports: not those of requests that the caller has meanwhile
+    taken away, nor those as a later request's of the same name."""
+    e = Engine()
+    a, b = e.add(9, "a"), e.add(3 if end == "pop_response" else 9, "b")
+    assert [e.step() for _ in range(3)] == [{}, {"a": 10, "b": 10}, {"a": 11, "b": 11}]
+    f = e.fork_request(a)  # the third token of each has been sampled: b's last, where it has three
+    assert e.get_generated_ids(f) == e.get_generated_ids(a) == [10, 11, 12]
+    getattr(e, end)(b)
+    again = e.add(2, "b")
+    assert e.step() == {"a": 12}
+    reported = {a: [], f: [], again: []}
+    while e.has_unfinished():
+        for rid, token in e.step().items():
+            reported[rid].append(token)
+    assert reported == {a: list(range(13, 19)), f: list(range(13, 19)), "b": [10, 11]}
+
+
+def test_nothing_is_left_to_do_when_what_was_read_early_is_gone():
+    e = Engine()
+    a = e.add(3)
+    for _ in range(3):
+        e.step()
+    with pytest.raises(ValueError, match="finished"):
+        e.fork_request(a)  # its last token was the one in flight
+    assert e.has_unfinished()  # to be reported
+    e.discard_request(a)
+    assert not e.has_unfinished()
