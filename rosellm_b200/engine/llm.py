@@ -174,6 +174,8 @@ class InferenceEngine:
             max_new_tokens=max_new_tokens, temperature=temperature, top_k=top_k, top_p=top_p,
             do_sample=do_sample, stop_on_eos=stop_on_eos, seed=seed,
         )
+        if request_id is None:
+            self._skip_names()
         req = self.scheduler.add_request(ids, params, request_id)
         self._requests[req.request_id] = req
         if req.status == FINISHED:
@@ -192,11 +194,18 @@ class InferenceEngine:
         if self._inflight is not None:  # the token of the step in flight is part of where the request stands
             inflight, self._inflight = self._inflight, None
             self._read_early = {**self._read_early, **self._resolve(inflight)}
+        if new_request_id is None:
+            self._skip_names()
         new = self.scheduler.fork(req, self.runner.fork, request_id=new_request_id, seed=seed, params=sampling_params)
         self._requests[new.request_id] = new
         if new.status == FINISHED:
             self._finished_ids.append(new.request_id)
         return new.request_id
+
+    def _skip_names(self) -> None:
+        """The number that names the next request without a name of its own is none that the caller has given one."""
+        while self.scheduler._next_id in self._requests:
+            self.scheduler._next_id += 1
 
     def has_unfinished(self) -> bool:
         return self.scheduler.has_unfinished() or self._inflight is not None or bool(self._read_early)

@@ -101,3 +101,21 @@ def test_nothing_is_left_to_do_when_what_was_read_early_is_gone():
     assert e.has_unfinished()  # to be reported
     e.discard_request(a)
     assert not e.has_unfinished()
+
+
+def test_a_fork_without_a_name_takes_no_others():
+    """Names that the engine gives itself are numbers that no request it knows of has, however the caller has numbered its own."""
+    e = Engine(seqs=6)
+    own = e.add(8, 1)
+    e.step(), e.step()
+    f = e.fork_request(own)
+    names = [own, f, e.fork_request(f), e.add(8, 4), e.add(8), e.add(8)]
+    assert len(set(names)) == 6 == len(e._requests)
+    while e.has_unfinished():
+        e.step()
+    assert sorted(e.pop_finished_ids()) == sorted(names) and all(e.pop_response(n).token_ids == list(range(10, 18)) for n in names)
+
+
+def test_names_of_requests_that_bring_none_are_counted():
+    e = Engine()
+    assert [e.add(), e.add(), e.add(3, "x"), e.add()] == [0, 1, "x", 3]
