@@ -176,3 +176,214 @@ def test_a_value_that_a_row_does_not_see_changes_nothing_for_it(K, each, heads, 
         outs.append(T.check_attention(K, each, heads, n_kv, dim, 16, dtype, touch=touch))
     ahead = 16 * block - (n - nq)
     assert 0 < ahead < nq and outs[0][:ahead].equal(outs[1][:ahead]) and not outs[0][ahead:].equal(outs[1][ahead:])
+
+
+# ---- the tcgen05 kernel: portions of 64 rows and more over contexts of 512 and more ----------------
+
+WIDE = [(700, 64), (1300, 130), (520, 520), (90, 70), (640, 1), (515, 2), (64, 64), (777, 191)]
+
+
+def check_wide(K, each, heads, n_kv, dim, page, **kw):
+    assert on_tcgen05(K, each, heads, n_kv, dim, page, kw.get("window"))
+    return T.check_attention(K, each, heads, n_kv, dim, page, BF16, **kw)
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,page", [(1, 1, 64, 16), (3, 1, 64, 48), (5, 1, 128, 80), (4, 2, 128, 32), (2, 2, 64, 112), (12, 1, 64, 64), (1, 1, 128, 4096)])
+def test_wide_portions(K, heads, n_kv, dim, page):
+    """Groups of heads that straddle a block of rows, pages whose number of blocks is no power of two, portions that end anywhere."""
+    check_wide(K, WIDE, heads, n_kv, dim, page)
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,page", [(2, 1, 64, 16), (2, 2, 128, 48)])
+@pytest.mark.parametrize("window", [448, 449, 511, 512, 700, 1100, 5000])
+def test_wide_portions_with_windows(K, heads, n_kv, dim, page, window):
+    check_wide(K, WIDE, heads, n_kv, dim, page, window=window)
+
+
+@pytest.mark.parametrize("spread", [0.0, 2.0, 4.0])
+def test_wide_portions_of_spread_values(K, spread):
+    check_wide(K, WIDE, 3, 1, 64, 16, spread=spread)
+
+
+@pytest.mark.parametrize("dim,n,nq,at", [(64, 700, 150, 640), (64, 700, 150, 100), (128, 600, 80, 599), (64, 1024, 512, 512), (128, 900, 130, 895)])
+@pytest.mark.parametrize("window", [None, 500])
+def test_wide_portions_and_nan(K, dim, n, nq, at, window):
+    """A value that is NaN reaches its dim of the rows that see the token, whatever the token weighs; a key that is NaN all of those rows of its head."""
+    heads = 2
+    sees = torch.tensor([at <= p and (window is None or at > p - window) for p in range(n - nq, n)])
+
+    def value(batch, q, pool, scales):
+        page, row = batch.row_of(0, at)
+        pool.view(torch.uint8)[page, 1, 0, row, [5, dim - 1]] = 0x7F
+
+    got = check_wide(K, [(n, nq)], heads, 2, dim, 16, window=window, touch=value).cpu()
+    assert torch.isnan(got[:, 5]).equal(sees) and torch.isnan(got[:, dim - 1]).equal(sees) and int(torch.isnan(got).sum()) == 2 * int(sees.sum())
+    gen = torch.Generator().manual_seed(2)
+    batch = P.Batch([(n, nq)], 16, seed=2)
+    pool, scales = T.cache_of(batch, 2, dim, gen)
+    page, row = batch.row_of(0, at)
+    pool.view(torch.uint8)[page, 0, 1, row, 7] = 0x7F
+    q = torch.randn(batch.tokens, heads * dim, generator=gen).to(BF16).to(DEV)
+    got = T.do_attention(K, batch, q, pool.to(DEV), scales.to(DEV), heads, window=window).cpu()
+    assert torch.isnan(got[:, dim:]).all(dim=1).equal(sees) and torch.isnan(got[:, dim:]).any(dim=1).equal(sees) and not torch.isnan(got[:, :dim]).any()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 48), (128, 64)])
+def test_wide_portions_without_some_pages(K, dim, page):
+    """Pages that are not there, first, in the middle of a tile and last, and a request without any: their keys are nobody's, and the status word says so."""
+    each = [(700, 130), (600, 64), (560, 70), (0, 66)]
+    batch = P.Batch([(max(n, 66), q) for n, q in each], page, seed=4)
+    batch.each = each
+    gen = torch.Generator().manual_seed(4)
+    pool, scales = T.cache_of(batch, 1, dim, gen)
+    q = torch.randn(batch.tokens, 2 * dim, generator=gen).to(BF16)
+    assert on_tcgen05(K, each, 2, 1, dim, page)
+    T.compare(T.do_attention(K, batch, q.to(DEV), pool.to(DEV), scales.to(DEV), 2), *P.attention(batch, q.double().unflatten(1, (2, dim)), P.values_of(pool),
+                                                                                             scales.double(), 2, dim ** -0.5), BF16)
+    K.check_status(DEV)
+    table = batch.table.clone()
+    table[batch.slots[0], 0], table[batch.slots[0], 300 // page], table[batch.slots[0], 699 // page] = -1, batch.n_pages, -7
+    table[batch.slots[2], :] = -1
+    batch.table = table
+    out = T.do_attention(K, batch, q.to(DEV), pool.to(DEV), scales.to(DEV), 2)
+    with pytest.raises(K.KernelError, match="page"):
+        K.check_status(DEV)
+    batch.table = torch.where(table >= batch.n_pages, -1, table)
+    want = P.attention(batch, q.double().unflatten(1, (2, dim)), P.values_of(pool), scales.double(), 2, dim ** -0.5)
+    T.compare(out, *want, BF16)
+    assert (out[batch.q_start[2]:] == 0).all()
+
+
+def test_wide_portions_give_the_same_bits_every_time(K):
+    batch = P.Batch([(1500, 200), (900, 70), (600, 64), (33, 1)], 32)
+    gen = torch.Generator().manual_seed(6)
+    pool, scales = (t.to(DEV) for t in T.cache_of(batch, 2, 128, gen))
+    q = torch.randn(batch.tokens, 8 * 128, generator=gen).to(BF16).to(DEV)
+    assert on_tcgen05(K, batch.each, 8, 2, 128, 32)
+    first = T.do_attention(K, batch, q, pool, scales, 8)
+    for _ in range(5):
+        assert T.do_attention(K, batch, q, pool, scales, 8).equal(first)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_wide_portions_captured(K, dim):
+    """A graph of the tcgen05 kernel and its join, captured at one length, serves longer and shorter contexts."""
+    batch = P.Batch([(2600, 100), (1800, 64)], 16)
+    gen = torch.Generator().manual_seed(5)
+    pool, scales = (t.to(DEV) for t in T.cache_of(batch, 2, dim, gen))
+    q = torch.randn(batch.tokens, 4 * dim, generator=gen).to(BF16).to(DEV)
+    a = batch.arrays(DEV)
+    out = torch.zeros(batch.tokens, 4 * dim, dtype=BF16, device=DEV)
+    sizes = dict(n_heads=4, span=600, n_tiles=3, max_q=100)
+    floats = K.kv8_attention_scratch(dtype=BF16, n_kv=2, head_dim=dim, page_size=16, **sizes)
+    assert floats > 0 and on_tcgen05(K, [(600, 100)], 4, 2, dim, 16)
+    scratch = torch.full((floats,), float("nan"), device=DEV)
+
+    def go():
+        K.kv8_attention(q, pool, scales, a["block_table"], a["q_start"], a["kv_len"], a["slots"], out, scale=dim ** -0.5, tiles=a["tiles"], scratch=scratch, **sizes)
+
+    go()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        go()
+    for lens in ([2600, 1800], [600, 500], [100, 64], [2601 - 16, 700]):
+        a["kv_len"].copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        b = P.Batch(list(zip(lens, (100, 64))), 16)
+        b.table, b.slots = batch.table, batch.slots
+        T.compare(out, *P.attention(b, q.cpu().double().unflatten(1, (4, dim)), P.values_of(pool), scales.cpu().double(), 4, dim ** -0.5), BF16)
+    K.check_status(DEV)
+
+
+# ---- through the engine, at contexts where all of these kernels run ---------------------------------
+
+def formulas(cfg, t, r, slot, ids, first, rounding=lambda x: x):
+    """Logits of ``ids[first:]`` in 64 bits with the keys and values that the cache holds; ``rounding``: of what a 16-bit engine stores between products."""
+    import test_kv8_engine_gpu as E
+
+    G, D, H, eps = E.P, cfg["n_embd"], cfg["n_head"], cfg.get("layer_norm_epsilon", 1e-5)
+    n, act = len(ids), E.P.activation_of(cfg.get("activation_function", "gelu_new"))
+    x = t["wte.weight"][torch.tensor(ids[first:])] + t["wpe.weight"][first:n]
+    for i in range(cfg["n_layer"]):
+        p = f"h.{i}."
+        h = rounding(G.layer_norm(x, t[p + "ln_1.weight"], t[p + "ln_1.bias"], eps))
+        q = rounding(h @ t[p + "attn.c_attn.weight"] + t[p + "attn.c_attn.bias"])[:, :D].view(-1, H, D // H)
+        kv, _ = E.cached(r, i, slot, n)
+        s = torch.einsum("qhd,khd->hqk", q, kv[:, 0]) * (D // H) ** -0.5
+        s = s.masked_fill(torch.arange(n)[None] > torch.arange(first, n)[:, None], float("-inf"))
+        o = rounding(torch.einsum("hqk,khd->qhd", torch.softmax(s, dim=-1), kv[:, 1]).reshape(-1, D))
+        x = rounding(x + o @ t[p + "attn.c_proj.weight"] + t[p + "attn.c_proj.bias"])
+        h = rounding(G.layer_norm(x, t[p + "ln_2.weight"], t[p + "ln_2.bias"], eps))
+        x = rounding(x + rounding(act(h @ t[p + "mlp.c_fc.weight"] + t[p + "mlp.c_fc.bias"])) @ t[p + "mlp.c_proj.weight"] + t[p + "mlp.c_proj.bias"])
+    return rounding(G.layer_norm(x, t["ln_f.weight"], t["ln_f.bias"], eps)) @ t["wte.weight"].t()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("graphs", [False, True])
+def test_long_contexts_through_the_engine(K, tmp_path, dtype, graphs):
+    """Prompts in portions on tcgen05, decoded tokens beside them and alone over contexts whose keys are shared out and joined, steps issued again from
+    launch lists with their scratch, graphs, and a fork.  Tolerances are those of the engine's other tests: 1e-4 of the logits' size in 32 bits, and in
+    16 bits three times what rounding the formulas' activations to bfloat16 does to these very logits."""
+    import test_kv8_engine_gpu as E
+    from rosellm_b200.config import GPT2Config
+    from rosellm_b200.weights import write_model_folder
+
+    folder = str(tmp_path / "long")
+    write_model_folder(GPT2Config(n_layer=2, n_embd=128, n_head=2, n_inner=256, vocab_size=500, n_positions=4608, layer_norm_epsilon=1e-5,
+                                  activation_function="gelu_new"), 7, folder, std=0.1, norm_affine="random")
+    cfg, t = E.P.load_folder(folder)
+    half = dtype == "bfloat16"
+    if half:
+        t = {k: (v.to(BF16).double() if v.dim() > 1 else v) for k, v in t.items()}
+    r = E.runner(folder, dtype, cuda_graphs=graphs, kv_cache_max_tokens=16384, max_batch_size=4, max_num_batched_tokens=2048)
+    rng = torch.Generator().manual_seed(3)
+    ids = [torch.randint(0, 500, (n,), generator=rng).tolist() for n in (2400, 2400, 700)]
+    assert K.kv8_on_tcgen05(K.BF16, 64, 64, 16, 1024)
+    assert K.kv8_attention_scratch(dtype=BF16 if half else F32, n_heads=2, n_kv=2, head_dim=64, page_size=16, span=2300, n_decode=1) > 0
+
+    def step(slots, at, counts, who=(0, 1, 2)):
+        """One step, each of whose last rows is compared with the formulas."""
+        entries = [E.entry(slots[i], ids[i][at[i]:at[i] + n], list(range(max(0, n - 80), n))) for i, n in zip(who, counts) if n]
+        logits = r.step(entries).clone()
+        row = 0
+        for i, n in zip(who, counts):
+            if n:
+                keep = min(n, 80)
+                at[i] += n
+                x = formulas(cfg, t, r, slots[i], ids[i][:at[i]], at[i] - keep)
+                limit = 1e-4 * max(1.0, float(x.abs().max()))
+                if half:
+                    limit = 3 * float((formulas(cfg, t, r, slots[i], ids[i][:at[i]], at[i] - keep, E.P.to_bfloat16_and_back) - x).abs().max())
+                off = float((logits[row:row + keep].cpu().double() - x).abs().max())
+                assert off <= limit, (i, n, at[i], off, limit)
+                row += keep
+        return logits
+
+    slots, at = [r.cache.new_request() for _ in ids], [0, 0, 0]
+    step(slots, at, (1024, 0, 0))
+    first = step(slots, at, (1024, 0, 0))
+    step(slots, at, (252, 0, 0))
+    step(slots, at, (1, 0, 600))
+    step(slots, at, (1, 0, 1))
+    ids[1][:2048] = ids[0][:2048]
+    before = r.launch_list_replays
+    step(slots, at, (0, 1024, 0))
+    again = step(slots, at, (0, 1024, 0))
+    # the same launches over other pages (a list that was noted before a buffer of the workspace grew is noted again)
+    assert r.launch_list_replays > before and again.equal(first)
+    step(slots, at, (1, 200, 1))
+    for _ in range(3):
+        step(slots, at, (1, 1, 1))
+    f = r.fork(slots[0])
+    slots.append(f)
+    ids.append(ids[0][:at[0]] + ids[2][:20])
+    at.append(at[0])
+    step(slots, at, (1, 2, 1), who=(0, 1, 3))
+    step(slots, at, (1, 1, 1, 1), who=(0, 1, 2, 3))
+    r.check_status()
+    for s in slots:
+        r.cache.release(s)
+    r.cache.check()
