@@ -76,10 +76,17 @@ __device__ __forceinline__ Work work_of(const AttnParams8& p, int entry) {
   const int group = p.n_heads / p.n_kv_heads;
   w.req = p.is_tiles ? p.items[2 * item] : p.items[item];
   const int t0 = p.is_tiles ? p.items[2 * item + 1] : 0;
+  // Blocks of 128 rows of heads that stand alone take two tiles of 64 queries at once, where the list has them next to one another: the first of them both,
+  // the second nothing.
+  int before[2] = {-1, 0}, next[2] = {-1, 0};
+  if (RB == 2 * TILE_QUERIES && group == 1 && p.is_tiles && p.row_blocks == 1) {
+    if (item > 0) before[0] = p.items[2 * item - 2], before[1] = p.items[2 * item - 1];
+    if (item + 1 < p.n_entries) next[0] = p.items[2 * item + 2], next[1] = p.items[2 * item + 3];
+  }
   const int qs = p.q_start[w.req], q_len = p.q_start[w.req + 1] - qs, kv_len = p.kv_len[w.req];
-  // (blocks of 128 rows of heads that stand alone take two tiles of 64 queries at once: the first of them both, the second nothing)
-  const bool doubled = RB == 2 * TILE_QUERIES && group == 1 && p.is_tiles;
-  const int n_q = doubled && t0 % (2 * TILE_QUERIES) != 0 ? 0 : min(!p.is_tiles ? 1 : doubled ? 2 * TILE_QUERIES : TILE_QUERIES, q_len - t0);
+  const bool first_half = t0 % (2 * TILE_QUERIES) == 0;
+  const bool paired = first_half ? next[0] == w.req && next[1] == t0 + TILE_QUERIES : t0 % TILE_QUERIES == 0 && before[0] == w.req && before[1] == t0 - TILE_QUERIES;
+  const int n_q = paired && !first_half ? 0 : min(!p.is_tiles ? 1 : paired ? 2 * TILE_QUERIES : TILE_QUERIES, q_len - t0);
   w.first_row = (entry - item * p.row_blocks) * RB;
   w.rows = min(RB, n_q * group - w.first_row);
   w.token0 = qs + t0;

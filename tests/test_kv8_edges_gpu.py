@@ -298,6 +298,27 @@ def test_wide_portions_captured(K, dim):
     K.check_status(DEV)
 
 
+@pytest.mark.parametrize("heads,n_kv,dim", [(1, 1, 64), (2, 2, 128), (2, 1, 64)])
+@pytest.mark.parametrize("tiles", [[(0, 0)], [(0, 64)], [(0, 64), (0, 0)], [(0, 128), (1, 0)], [(0, 64), (0, 128), (1, 64)], [(1, 0), (0, 0), (0, 128), (0, 64)], [(0, 0), (1, 64)]])
+def test_wide_portions_of_some_tiles(K, heads, n_kv, dim, tiles):
+    """A list that names some of a request's tiles, in any order: the rows of those are written, the others stay (two neighbours may share a block of rows)."""
+    each = [(700, 200), (600, 128)]
+    batch = P.Batch(each, 16, seed=8)
+    gen = torch.Generator().manual_seed(8)
+    pool, scales = T.cache_of(batch, n_kv, dim, gen)
+    q = torch.randn(batch.tokens, heads * dim, generator=gen).to(BF16)
+    assert on_tcgen05(K, each, heads, n_kv, dim, 16)
+    want = P.attention(batch, q.double().unflatten(1, (heads, dim)), P.values_of(pool), scales.double(), heads, dim ** -0.5)
+    batch.tiles = tiles
+    out = T.do_attention(K, batch, q.to(DEV), pool.to(DEV), scales.to(DEV), heads)
+    K.check_status(DEV)
+    named = torch.zeros(batch.tokens, dtype=torch.bool)
+    for r, t in tiles:
+        named[batch.q_start[r] + t:batch.q_start[r] + min(t + 64, each[r][1])] = True
+    assert (out[~named.to(DEV)] == 7).all()
+    T.compare(out[named.to(DEV)], *(x[named] for x in want), BF16)
+
+
 # ---- through the engine, at contexts where all of these kernels run ---------------------------------
 
 def formulas(cfg, t, r, slot, ids, first, rounding=lambda x: x):
