@@ -120,6 +120,13 @@ __device__ __forceinline__ float ex2_small(float x) {
   return y;
 }
 
+// 1 / x to 2^-23, without the branches of a rounded division.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -906,7 +913,7 @@ __global__ __launch_bounds__(160, Shapes<DH, F32, NR>::AT_ONCE) void kv8_attenti
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         // (2^-15 / l and 2^(t - m) one after the other: their product may be too small)
-        const float inv = l[j][i] == 0.f ? 0.f : 3.0517578125e-05f / l[j][i], up = ex2(st.t[j][i] - m[j][i]);
+        const float inv = l[j][i] == 0.f ? 0.f : 3.0517578125e-05f * reciprocal(l[j][i]), up = ex2(st.t[j][i] - m[j][i]);
 #pragma unroll
         for (int t = 0; t < S::MT; ++t) {
           st.o[j][t][i] = st.o[j][t][i] * inv * up;
@@ -983,20 +990,31 @@ __global__ __launch_bounds__(128) void kv8_join_kernel(const AttnParams8 p) {
   for (int i = threadIdx.x; i < n_rows * quads; i += 128) {
     const int row = row0 + i / quads, d = i % quads * 4;
     float m = NOTHING, l = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(k, row) * 2);
-      const float most = fmaxf(m, ml.x);
-      l = l * ex2(m - most) + ml.y * ex2(ml.x - most);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);  // the mean so far
+    for (int k = 0; k < parts; k += 4) {         // four parts' loads on their way at once
+      float2 ml[4];
+      float4 part[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const size_t at = part_row(k + j, row);
+        const bool there = k + j < parts;
+        ml[j] = there ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : make_float2(NOTHING, 0.f);
+        part[j] = there ? *reinterpret_cast<const float4*>(p.part_o + at * p.head_dim + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const float most = fmaxf(fmaxf(m, ml[0].x), fmaxf(ml[1].x, fmaxf(ml[2].x, ml[3].x)));
+      float w[4], before = l * ex2(m - most);
+      l = before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = ml[j].y * ex2(ml[j].x - most), l += w[j];
       m = most;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < parts; ++k) {
-      const size_t at = part_row(k, row);
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float f = ml.y * ex2(ml.x - m) * inv;
-      const float4 a = *reinterpret_cast<const float4*>(p.part_o + at * p.head_dim + d);
-      o.x += a.x * f, o.y += a.y * f, o.z += a.z * f, o.w += a.w * f;
+      const float inv = l == 0.f ? 0.f : reciprocal(l);
+      before *= inv;
+      o.x *= before, o.y *= before, o.z *= before, o.w *= before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = w[j] * inv;
+        o.x += part[j].x * f, o.y += part[j].y * f, o.z += part[j].z * f, o.w += part[j].w * f;
+      }
     }
     store4<F32>(p.out, out_at(p, rows, row) + d, o.x, o.y, o.z, o.w);
   }

@@ -623,7 +623,7 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
         const float4 a = ml[row], b = ml[128 + row];
         const float top = fmaxf(a.x, b.x), fa = ex2(a.x - top), fb = ex2(b.x - top), sum = a.y * fa + b.y * fb;
         // means (which are no larger than the largest value; a sum may be); the powers of two in halves, of which neither is too small or too large
-        const float by = sum == 0.f ? 0.f : 4.8828125e-4f / sum, ua = ex2(0.5f * (a.x - top + a.z)), ub = ex2(0.5f * (b.x - top + b.z));  // 2^-11
+        const float by = sum == 0.f ? 0.f : 4.8828125e-4f * reciprocal(sum), ua = ex2(0.5f * (a.x - top + a.z)), ub = ex2(0.5f * (b.x - top + b.z));  // 2^-11
         const size_t part_row = (size_t)s.part * TC_ROWS + row;
         const size_t to = s.part < 0 ? (size_t)(s.token0 + q) * p.out_stride + (size_t)h * DH : part_row * DH;
 #pragma unroll 1
