@@ -14,14 +14,14 @@
 // and 2c+1 are keys c and c+4, so that neighbouring lanes read neighbouring rows of V.  P^T is S^T's fragment transposed in registers (movmatrix).
 //
 // Scales: the 16 keys of a block share a key scale, by which their scores are multiplied.  A block of values is one inner step of P V, so its
-// probabilities are multiplied by its scale.  The outputs therefore have a maximum of their own beside the softmax's: T, the largest score + log2(value
-// scale) that the row has seen; probabilities enter P V as halves of 2^(score + log2 scale - T + 15).  The key that moves the output most thus
-// stands at 2^15 (exactly, where it alone matters) whatever the scales are, keys down to 2^-29 of it keep all of their 11 bits (relative error 2^-11, against
-// 2^-8 of a bfloat16 output), and none is off by more than 2^-40 of it.  What a row does not see has no part in T.  (Probabilities against the largest
-// scale so far, which may belong to keys of no weight or out of sight, lost bits from a ratio of 2^-18 on and everything at 2^-40.)  In 32 bits T is
-// rounded up: changes of it are exact then.  Q is brought to halves row by row with a power of two that puts its largest entry at 2^14 (a bfloat16 fits exactly,
-// within 2^-28 of the row's largest); in 32 bits Q and P are two halves each, a value and what its rounding left, so that products
-// are exact to 2^-22.  Sums, maxima and outputs are float32.
+// probabilities are multiplied by its scale.  The outputs therefore have a maximum of their own beside the softmax's: T, the largest score +
+// log2(value scale) that the row has seen; probabilities enter P V as halves of 2^(score + log2 scale - T + 15).  The key that moves the output most
+// thus stands at 2^15 (exactly, where it alone matters) whatever the scales are, keys down to 2^-29 of it keep all of their 11 bits (relative error
+// 2^-11, against 2^-8 of a bfloat16 output), and none is off by more than 2^-40 of it.  What a row does not see has no part in T.  (Probabilities
+// against the largest scale so far, which may belong to keys of no weight or out of sight, lost bits from a ratio of 2^-18 on and everything at
+// 2^-40.)  In 32 bits both maxima are rounded up: all factors that follow from them are exact then.  Q is brought to halves row by row with a power
+// of two that puts its largest entry at 2^14 (a bfloat16 fits exactly, within 2^-28 of the row's largest); in 32 bits Q and P are two halves each, a
+// value and what its rounding left, so that products are exact to 2^-22.  Sums, maxima and outputs are float32.
 #pragma once
 #include "kv8.cuh"
 #include "tc_common.cuh"
@@ -391,7 +391,7 @@ __device__ __forceinline__ void use_scores(const Sight sight, State<DH, NR>& st,
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
         t = fmaxf(st.t[n][i], F32 ? ceilf(t) : t);
-        const float m = fmaxf(st.m[n][i], top[n][i]);
+        const float m = fmaxf(st.m[n][i], F32 ? ceilf(top[n][i]) : top[n][i]);
         st.l[n][i] *= ex2(st.m[n][i] - m);
         turn[i] = ex2(st.t[n][i] - t);
         st.m[n][i] = m, st.t[n][i] = t;
