@@ -153,8 +153,11 @@ __global__ __launch_bounds__(TC_THREADS, 1) void kv8_attention_tc_kernel(const A
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // Kernels behind are let in by this warp, when the block has its tensor memory: one that takes some before it waits for this kernel could otherwise
+    // stand on the SM first, and each would wait for the other.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
-  pdl_begin();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // what the entries before each come to for one head, in the place of the first keys
   int* before = reinterpret_cast<int*>(smem + L::K);
   for (int e = threadIdx.x; e < p.n_entries; e += TC_THREADS) {

@@ -24,6 +24,16 @@ def test_the_next_block_is_asked_for_when_all_lanes_have_read_the_answer():
     assert "__syncwarp();" in asking[0].split("ask_for_block(")[0]
 
 
+def test_kernels_behind_are_let_in_when_a_block_has_its_tensor_memory():
+    """A kernel that takes tensor memory and then waits for the kernels ahead may stand beside a block of those that has not taken its own yet, if that
+    block has let it in before: both would wait for good."""
+    source = open(os.path.join(CSRC, "kv8_attention_tc.cuh")).read()
+    kernel = source[source.index("void kv8_attention_tc_kernel("):source.index("int launch_attention_tc(")]
+    assert "pdl_begin(" not in kernel and kernel.count("launch_dependents") == 1 == kernel.count("tcgen05.alloc") == kernel.count("griddepcontrol.wait")
+    own = re.search(r"if \(warp == 16\) \{(.*?)\n  \}", kernel, re.S).group(1)
+    assert own.index("tcgen05.alloc") < own.index("launch_dependents") and kernel.index("launch_dependents") < kernel.index("griddepcontrol.wait")
+
+
 def test_a_pool_without_pages_is_refused():
     """The tcgen05 kernel reads the pool's first page in the place of one that is not there (its keys are hidden): there has to be one."""
     at = torch.zeros(64).data_ptr()
