@@ -568,8 +568,8 @@ __device__ __forceinline__ bool read_answer(uint32_t answer, int& x) {
 // 1: the tiles of all units in a row, and in front of each unit's the cost of beginning one, are cut into as many equal runs as blocks stand on the device
 // at once (but runs of at least p.cost + 4 tiles, or of up to p.cost + 16 where there is one for each SM), whatever the lengths.  A unit that a
 // run has the whole of goes to the output; of others, a run has at most two, and kv8_join_kernel joins their parts.  32 contexts of up to 16384 tokens, 8 heads of 128: 114 us in parts of 1536
-// keys that blocks take over from one another, which leaves the last of them waiting for the longest; 102 so, of 85 of traffic.
-// What bounds it where units are short (64 decoded tokens of 25 heads of 64 and up to 1023 keys: 39 us, 16.6 of traffic) is latency: a block takes
+// keys that blocks take over from one another, which leaves the last of them waiting for the longest; 100 so, of 85 of traffic.
+// What bounds it where units are short (64 decoded tokens of 25 heads of 64 and up to 1023 keys: 40 us, 16.6 of traffic) is latency: a block takes
 // 17,000 cycles for a unit of ten tiles, of which its warps compute 6,600; fifteen warps an SM issue in 29 % of the cycles.
 //
 // The fetching warp tells the others what comes next by a segment, two of which may be open, and lays the queries out for them (decoded tokens: the

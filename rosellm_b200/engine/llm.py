@@ -187,7 +187,8 @@ class InferenceEngine:
         """A second request that goes on from where a running one stands: the same prompt, the same tokens generated so far, the same cache (whole
         pages are shared, the last one is copied), and a random stream of its own from here on.  ``sampling_params``: how it goes on (default: as
         the first one does; ``max_new_tokens`` counts the tokens generated so far as well).  Raises ``ValueError`` for a request that is
-        not running (waiting, or finished), and ``OutOfPages`` when there is no slot or no page for another."""
+        not running (waiting, or finished) and when as many requests run as the engine takes, and ``OutOfPages`` when there is no slot or no page for another.
+        Tokens of a step in flight are read first, and reported by the next ``step`` for the requests that are still there then."""
         req = self._requests[request_id]
         if new_request_id is not None and new_request_id in self._requests:
             raise ValueError(f"request {new_request_id!r} exists already")

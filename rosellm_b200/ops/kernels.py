@@ -2223,8 +2223,8 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
 def kv8_on_tcgen05(code: int, rows: int, dh: int, page_size: int, span: int) -> bool:
     """Whether items of up to ``rows`` rows (queries times the heads of a group) run on the tcgen05 kernel (csrc/kv8_attention_tc.cuh): those that
     fill half of its 128 rows, over contexts long enough to pay for its beginning.  Measured on B200, us, mma.sync / tcgen05: 32 heads on 8 of 128, 16
-    queries x 16 of 1000 70.8 / 54.0, x 8 of 4000 77 / 71, 8 queries x 8 of 4000 (32 rows) 40.7 / 44.7, 12 x 32 of 300 (48 rows) 36.8 / 60.7, prompts
-    of 4 x 512 75 / 62, 512 of 1024 59.8 / 41.6; 12 heads of 64, prompts of 2 x 1024 53.0 / 35.1, 8 x 256 16.4 / 24.9, one of 100 10.7 / 12.9."""
+    queries x 16 of 1000 75 / 54, x 8 of 4000 85 / 70, 8 queries x 8 of 4000 (32 rows) 42.6 / 44.4, 12 x 32 of 300 (48 rows) 39.2 / 59.7, prompts
+    of 4 x 512 82 / 62, 512 of 1024 68 / 42; 12 heads of 64, prompts of 2 x 1024 57.0 / 35.7, 8 x 256 16.7 / 24.9, one of 100 11.2 / 13.1."""
     return code == BF16 and dh in (64, 128) and rows >= 64 and span >= 512 and page_size <= 4096
 
 
@@ -2233,8 +2233,8 @@ KV8_MOST_ENTRIES = 4096  # blocks of rows whose keys are shared evenly: their nu
 
 def _kv8_by_units(dh: int, span: int) -> bool:
     """Whether units are short enough for a block each: up to 256 KB of keys and values.  Measured on B200, us, by units / shared evenly: 12 heads of
-    64, one request of 700 keys 8.7 / 11.8, 16 of up to 1024 11.8 / 16.9, 32 of 512 9.1 / 17.2, 25 heads, 64 of 1023 38.8 / 40.1; 16 heads, 4 of 2048
-    15.5 / 15.1.  8 heads of 128, 256 of 1024 71.1 / 69.8, 16 of 2048 28.5 / 23.3, 64 of 2048 57.9 / 37.0, 32 of 16384 221 / 100."""
+    64, one request of 700 keys 9.0 / 11.9, of 2048 15.8 / 12.0, 16 of up to 1024 12.0 / 17.6, 32 of 512 9.4 / 17.8, 25 heads, 64 of 1023 40.4 / 41.5; 16 heads, 4 of 2048
+    15.9 / 15.0.  8 heads of 128, 256 of 1024 66.6 / 66.6, 16 of 2048 29.6 / 22.7, 64 of 2048 61.3 / 36.8, 32 of 16384 243 / 99."""
     return span * 2 * dh <= 256 << 10
 
 
@@ -2269,8 +2269,8 @@ def kv8_attention(q, pool, scales, block_table, q_start, kv_len, slots, out, *, 
     (csrc/kv8_attention.cuh).
 
     ``q`` [tokens, heads * head dim] float32 or bfloat16 (a view with a row stride), ``out`` the same shape and type (rows at multiples of
-    16 bytes).  ``tiles`` int32 [n_tiles, 2]: (request, first query) of every 64 queries of the requests that bring several (``max_q``: the most
-    that one of them brings), ``decode_reqs`` int32 [n_decode]: the requests that bring one.  Rows of ``out`` that belong to
+    16 bytes).  ``tiles`` int32 [n_tiles, 2]: (request, first query) of 64 queries each of the requests that bring several, in any order, though neighbours next
+    to one another are quickest (``max_q``: the most that one of them brings), ``decode_reqs`` int32 [n_decode]: the requests that bring one.  Rows of ``out`` that belong to
     neither are left as they are.  A query without a key in sight (``kv_len`` 0, a negative slot, which is padding, or pages missing, which sets the
     status word) gets zeros.
     ``span``: the longest context of these requests; it decides how their keys are shared out over blocks, not which keys
