@@ -204,7 +204,9 @@ struct Shapes {
   static constexpr int MT = DH / 16;                // row tiles of O^T
   static constexpr int QPARTS = F32 ? 2 : 1;        // halves of a query entry
   static constexpr int TB = DH <= 64 ? 4 : DH <= 128 ? 2 : 1;  // blocks of 16 keys of a tile: 4 to 8 KB of keys and values
-  static constexpr bool Q_IN_REGS = KSTEPS * QPARTS * NR <= 16;
+  // Q's fragments in registers, else read from shared memory step by step: with two eights of rows a head of 128 has none left for them (measured, us, in
+  // registers / not: 1024 queries of 4096, 32 heads on 8, 395 / 347, 8 x 5 queries of 20001 92 / 83, 12 heads of 64 in 32 bits, 2 x 1024, 84.8 / 80.2).
+  static constexpr bool Q_IN_REGS = KSTEPS * QPARTS * NR <= (NR == 1 ? 16 : 8);
   static constexpr int Q_BYTES = NR * QPARTS * KSTEPS * 256;
   static constexpr int CHUNK = DH % 64 == 0 ? 16 : 8;  // bytes of a key's row that a lane takes at once; the four lanes of a row take neighbouring ones
   static constexpr int AT_ONCE = NR == 1 && DH <= 128 && !F32 ? 3 : NR == 1 || DH <= 160 ? 2 : 1;  // blocks of threads on an SM (registers)

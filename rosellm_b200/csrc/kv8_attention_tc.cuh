@@ -17,8 +17,7 @@
 //
 // What bounds it: 128 x 128 exponentials take 1024 cycles of an SM, the products of a tile 1024 (head 128) or 512; turning 32 KB of codes into
 // halves takes 260 issue slots a scheduler.  Work is shared over the SMs in equal runs of tiles, as there.  Measured: a tile takes 3,350 cycles at
-// head 128; 2048 queries of 32 heads (8 of keys) after 16,384 776 us, 0.39 of the measured rate of a product of that many operations; on mma.sync 2,562 before
-// values were scaled as they are now.
+// head 128; 2048 queries of 32 heads (8 of keys) after 16,384 776 us, 0.39 of the measured rate of a product of that many operations; on mma.sync 2,608.
 #pragma once
 #include "kv8_attention.cuh"
 

@@ -2223,8 +2223,8 @@ def _kv8_plan(code: int, is_tiles: int, n_items: int, queries: int, n_heads: int
 def kv8_on_tcgen05(code: int, rows: int, dh: int, page_size: int, span: int) -> bool:
     """Whether items of up to ``rows`` rows (queries times the heads of a group) run on the tcgen05 kernel (csrc/kv8_attention_tc.cuh): those that
     fill half of its 128 rows, over contexts long enough to pay for its beginning.  Measured on B200, us, mma.sync / tcgen05: 32 heads on 8 of 128, 16
-    queries x 16 of 1000 75 / 54, x 8 of 4000 85 / 70, 8 queries x 8 of 4000 (32 rows) 42.6 / 44.4, 12 x 32 of 300 (48 rows) 39.2 / 59.7, prompts
-    of 4 x 512 82 / 62, 512 of 1024 68 / 42; 12 heads of 64, prompts of 2 x 1024 57.0 / 35.7, 8 x 256 16.7 / 24.9, one of 100 11.2 / 13.1."""
+    queries x 16 of 1000 70 / 54, x 8 of 4000 78 / 70, 8 queries x 8 of 4000 (32 rows) 39.1 / 44.4, 12 x 32 of 300 (48 rows) 37.2 / 59.9, prompts
+    of 4 x 512 73 / 62, 512 of 1024 61 / 42; 12 heads of 64, prompts of 2 x 1024 56.7 / 35.7, 8 x 256 16.7 / 24.7, one of 100 11.1 / 13.0."""
     return code == BF16 and dh in (64, 128) and rows >= 64 and span >= 512 and page_size <= 4096
 
 
