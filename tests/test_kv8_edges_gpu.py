@@ -178,6 +178,25 @@ def test_a_value_that_a_row_does_not_see_changes_nothing_for_it(K, each, heads, 
     assert 0 < ahead < nq and outs[0][:ahead].equal(outs[1][:ahead]) and not outs[0][ahead:].equal(outs[1][ahead:])
 
 
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_a_query_that_is_not_finite_is_its_own_row_s_matter(K, shape):
+    """A NaN in one token's one head: that row is NaN, all the others are what they were, bit by bit."""
+    each, heads, n_kv, dim, page, dtype = SHAPES[shape]
+    batch = P.Batch(each, page, seed=9)
+    gen = torch.Generator().manual_seed(9)
+    pool, scales = (t.to(DEV) for t in T.cache_of(batch, n_kv, dim, gen))
+    q = torch.randn(batch.tokens, heads, dim, generator=gen).to(dtype).to(DEV)
+    want = T.do_attention(K, batch, q.flatten(1), pool, scales, heads).view_as(q)
+    for token, head in ((0, heads - 1), (batch.tokens // 2, 0)):
+        spoilt = q.clone()
+        spoilt[token, head, dim // 3] = float("nan")
+        got = T.do_attention(K, batch, spoilt.flatten(1), pool, scales, heads).view_as(q)
+        assert torch.isnan(got[token, head]).all()
+        got[token, head] = want[token, head]
+        assert got.equal(want)
+    K.check_status(DEV)
+
+
 # ---- the tcgen05 kernel: portions of 64 rows and more over contexts of 512 and more ----------------
 
 WIDE = [(700, 64), (1300, 130), (520, 520), (90, 70), (640, 1), (515, 2), (64, 64), (777, 191)]
