@@ -158,7 +158,8 @@ namespace rl {
 // tensor-memory allocation, index arithmetic) thus overlap the tail of the previous kernel.
 //
 // What a kernel may read before its wait.  Kernel N starts once every block of kernel N-1 has
-// passed its launch_dependents, which is at N-1's top: so N's part before the wait can run
+// passed its launch_dependents, which is at N-1's top (where the block takes tensor memory: behind
+// that, or a later kernel's block could take it and wait for one that waits for it): so N's part before the wait can run
 // beside the body of N-1, and, N-1 itself having started that early, beside N-2 and earlier
 // kernels.  Before its wait a kernel therefore reads only memory that no kernel of the same
 // sequence of launches writes: weights and norm scales, the step's description (copied to the

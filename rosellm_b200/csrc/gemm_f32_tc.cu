@@ -114,7 +114,6 @@ __global__ __launch_bounds__(THREADS, 1) void gemm_f32_tc_kernel(const __grid_co
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int m_tiles = (p.M + BM - 1) / BM, units = m_tiles * ((p.N + BN - 1) / BN), kbs = (p.K + BK - 1) / BK;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
       tc::mbar_init(full_bar(s), 1);
@@ -135,6 +134,9 @@ __global__ __launch_bounds__(THREADS, 1) void gemm_f32_tc_kernel(const __grid_co
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)), "r"(TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // Kernels behind are let in by this warp, when the block has its tensor memory: one that takes some before it waits for this kernel could otherwise stand
+    // on the SM first, and each would wait for the other.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

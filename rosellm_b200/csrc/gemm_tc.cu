@@ -138,7 +138,6 @@ __global__ __launch_bounds__(PTHREADS, 1) void gemm_tc_persistent_kernel(const _
   const int num_kb = (p.K + BK - 1) / BK;
   const uint32_t acc_stride = (uint32_t)p.tmem_cols / 2;
   RL_PHASE(0);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < PSTAGES; ++s) {
@@ -168,6 +167,9 @@ __global__ __launch_bounds__(PTHREADS, 1) void gemm_tc_persistent_kernel(const _
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // Kernels behind are let in by this warp, when the block has its tensor memory: one that takes some before it waits for this kernel could otherwise stand
+    // on the SM first, and each would wait for the other.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   if constexpr (PAIR) {

@@ -76,7 +76,6 @@ __global__ __launch_bounds__(RTHREADS) void gemm_tc_rows_kernel(
   const int kb0 = rank * cut.kb_per;
   const int nkb = min(num_kb - kb0, cut.kb_per);  // > 0: no part of K is empty
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < cut.stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -93,6 +92,9 @@ __global__ __launch_bounds__(RTHREADS) void gemm_tc_rows_kernel(
                  "r"((uint32_t)cut.tmem_cols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // Kernels behind are let in by this warp, when the block has its tensor memory: one that takes some before it waits for this kernel could otherwise stand
+    // on the SM first, and each would wait for the other.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -34,6 +34,14 @@ def test_kernels_behind_are_let_in_when_a_block_has_its_tensor_memory():
     assert own.index("tcgen05.alloc") < own.index("launch_dependents") and kernel.index("launch_dependents") < kernel.index("griddepcontrol.wait")
 
 
+@pytest.mark.parametrize("name", sorted(f for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")) and "tcgen05.alloc" in open(os.path.join(CSRC, f)).read()))
+def test_tensor_memory_comes_first_in_every_kernel_that_takes_some(name):
+    """The same of the products and the attention that stand beside it on an SM."""
+    source = open(os.path.join(CSRC, name)).read()
+    assert source.count("launch_dependents;") == 1
+    assert source.rindex("tcgen05.alloc") < source.index("launch_dependents;")
+
+
 def test_a_pool_without_pages_is_refused():
     """The tcgen05 kernel reads the pool's first page in the place of one that is not there (its keys are hidden): there has to be one."""
     at = torch.zeros(64).data_ptr()
